@@ -353,6 +353,19 @@ int q_attention_prefill(const void* d_q, const q_kv_layout_t* kv, const int32_t*
                         void* d_out, int batch, int T, int n_q_heads, float scale,
                         void* stream);
 
+/* ---- attention over a part of the keys --------------------------------------
+ * (No reference counterpart.) d_pos: int32[1] for all sequences, or with pos_per_seq != 0
+ * int32[batch]. Positions, tables, queries and keys may come from the launch right before; nothing
+ * outside the block table's rows is read, whatever the position says, and no page that holds no visible key (the
+ * table may say anything there). What pages hold in places nobody sees may be anything, NaN too.
+ *
+ * q_attention_window: q_attention under a sliding window with sinks. Row (b, t, head) sits at
+ * p = pos + t and attends to keys j <= p with j > p - window or j < sinks. d_q [batch*T][n_q][128],
+ * T * n_q / n_kv <= 32; one launch, no scratch. A row that sees no key (a negative position) gives zeros. */
+int q_attention_window(const void* d_q, const q_kv_layout_t* kv, const int32_t* d_pos, int pos_per_seq,
+                       void* d_out, int batch, int T, int n_q_heads, int window, int sinks, float scale,
+                       void* stream);
+
 /* The three kernels above for the single-token decode step in ONE launch:
  * engine/kernels/decode_fused.py:172-210 (head norm + RoPE + K/V write into the page
  * slot *d_pos) + engine/kernels/small_query_attention.py:113-158 (split-KV attention and

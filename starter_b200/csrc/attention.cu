@@ -16,7 +16,7 @@
 // Every mbarrier wait is bounded: when it runs out the thread records a code in
 // the device status word and the CTA stops consuming, so a lost copy can never
 // hang the GPU.
-#include "common.cuh"
+#include "mma.cuh"
 
 extern int g_attn_no_cluster;   // q_set_option "attn_no_cluster": merge splits through global memory
 
@@ -79,32 +79,6 @@ __device__ __forceinline__ void copy_tile(unsigned char* stage, const char* k, c
   mbar_expect_tx(bar, 2 * bytes);
   bulk_g2s(smem_u32(stage), k, bytes, bar);
   bulk_g2s(smem_u32(stage) + TILE_BYTES, v, bytes, bar);
-}
-__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2,
-                                        uint32_t& r3) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr));
-}
-__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2,
-                                          uint32_t& r3) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr));
-}
-__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// 8 x 8 bf16 matrix, a lane's pair (row lane / 4, columns 2 (lane % 4) ..), transposed.
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
-  uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
-  return r;
 }
 __device__ __forceinline__ void consumer_sync() {
   asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS * 32) : "memory");

@@ -1,0 +1,538 @@
+// Attention of a few query rows per kv head (1-8 tokens per sequence, at most 32 rows) over a part of a
+// paged cache: a sliding window with first tokens kept (sinks), and both halves of the attention of a
+// batch that shares a prefix - few rows over the prefix, and every sequence's own keys, joined with the
+// partial results of the prefix.
+//
+//   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  s_j = scale q . k_j,  m = max_j s_j
+//
+// over the keys j that the row sees. A cluster of CTAs shares one (sequence, kv head): the pages that hold
+// a visible key are dealt out evenly, every CTA keeps a running maximum, sum and weighted sum, and the parts
+//   (m, l, O) (+) (m', l', O') = (M, e^(m-M) l + e^(m'-M) l', e^(m-M) O + e^(m'-M) O'),  M = max(m, m')
+// are joined in the cluster's shared memory, in a fixed order.
+//
+// Bound by the bytes of the visible keys at long windows, by latencies at short ones (position -> pages ->
+// keys -> join is a chain of memory round trips); hence one launch, and of a page only the rows somebody sees
+// are copied: a window with 4 sinks brings 4 rows of its first page.
+//
+// Keys are the M dimension of the MMAs, query rows (NT tiles of 8) the N dimension: S^T = K Q^T, O^T = V^T P^T,
+// as in the decode attention, so that few rows leave no accumulator empty. DG groups of four warps take a tile of
+// 64 keys each, a warp 16 keys. Cast boundaries as there: fp32 scores and statistics, P rounded to bf16 for
+// P V (the tensor cores' operand type), fp32 sums, one rounding of the result.
+//
+// Rows of a page that no query row sees may hold anything: their scores are replaced, their values cleared.
+#include "mma.cuh"
+#include "tc.cuh"
+#include "attn_parts.cuh"
+
+int* q_attn_status_addr();
+
+namespace {
+
+constexpr int ROW_TILE = Q_PAGE_TOKENS * 256;      // bytes of a K or V page tile
+constexpr int ROW_STAGE = 2 * ROW_TILE;
+constexpr int ROW_LD = 136;                        // floats of a row of the warps' merge area (rows on other banks)
+constexpr int MAX_SPLITS = 8;                      // CTAs of a cluster (the portable size)
+
+struct RowsArgs {
+  const bf16* q;
+  const char* kpool;
+  const char* vpool;
+  const int32_t* table;
+  const int32_t* pos;        // flat: the number of keys
+  bf16* out;                 // final rows, or
+  AttnParts parts;           // ... written (write_parts) or joined (parts.splits > 0)
+  int pages_per_seq, pos_step, T, G, nq, nkv, window, sinks, share, stages;
+  float scale_log2;
+  bool flat;                 // every row sees keys [0, *pos): rows over a shared prefix
+  bool write_parts;
+  bool early;                // keys and queries are older than the launch before this one
+};
+
+// What a sequence's rows see, and in which pages it lies.
+struct Seen {
+  int pos, lim, low;         // position of row 0; newest visible key + 1; oldest key of the first row's window
+  int sink_pages, window_page, pages;
+};
+
+__device__ __forceinline__ Seen seen_of(const RowsArgs& a, int b) {
+  Seen s;
+  const int room = a.pages_per_seq * Q_PAGE_TOKENS;
+  int p = __ldcg(a.pos + (size_t)b * a.pos_step);
+  if (a.flat) p = max(0, p) - a.T;                               // row T-1 is then the newest key
+  // positions outside the pages see what there is: nothing outside the table is read
+  s.pos = a.flat ? min(p, room - a.T) : min(max(p, -a.T), room);
+  s.lim = min(max(s.pos + a.T, 0), room);
+  s.low = a.flat ? 0 : min(max(0, s.pos - a.window + 1), s.lim);
+  s.sink_pages = (min(a.sinks, s.lim) + Q_PAGE_TOKENS - 1) / Q_PAGE_TOKENS;
+  s.window_page = max(s.sink_pages, s.low / Q_PAGE_TOKENS);
+  s.pages = s.sink_pages + max(0, (s.lim + Q_PAGE_TOKENS - 1) / Q_PAGE_TOKENS - s.window_page);
+  return s;
+}
+__device__ __forceinline__ int page_of(const Seen& s, int i) {
+  return i < s.sink_pages ? i : i - s.sink_pages + s.window_page;
+}
+
+__device__ __forceinline__ void copy_rows(uint32_t dst, const char* src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t remote_addr(uint32_t local, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
+  return r;
+}
+
+template <int NT, int DG>
+__global__ void __launch_bounds__((4 * DG + 1) * 32, (NT <= 2 && DG == 1) ? 2 : 1)
+k_attn_rows(const RowsArgs a, int* status) {
+  constexpr int DC = 4 * DG;                       // consumer warps
+  constexpr int DT = (DC + 1) * 32;
+  constexpr int SETS = NT == 1 ? 4 : NT == 2 ? 2 : 1;      // accumulators of a row tile's Q K^T
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const int NS = a.stages;
+  unsigned char* stages = smem;
+  unsigned char* qtile = smem + NS * ROW_STAGE;                            // NT * 8 rows of 256 B
+  uint64_t* bars = reinterpret_cast<uint64_t*>(qtile + NT * 8 * 256);      // full[NS], empty[NS]
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * NS);
+  float* recv = reinterpret_cast<float*>(bars + 2 * NS + 2);               // [splits][share] sums, then [splits][R][2]
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int b = blockIdx.y / a.nkv, kh = blockIdx.y - b * a.nkv;
+  const int R = a.T * a.G;
+  const int rank = (int)cluster_rank(), S = (int)cluster_size();
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(smem_u32(&bars[i]), 1);
+      mbar_init(smem_u32(&bars[NS + i]), 4);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  __syncthreads();
+  // (waited for before the first store into another CTA's memory: that CTA has to be running)
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  if (!a.early) pdl_wait();      // position, table, queries and keys may come from the launch before
+  // (after the wait: what follows may then read early whatever the launches before this one wrote)
+  pdl_launch_dependents();
+
+  const Seen seen = seen_of(a, b);
+  // pages are dealt out evenly over all splits of the grid's row
+  const int parts = gridDim.x, part = blockIdx.x;
+  const int each = seen.pages / parts, more = seen.pages - each * parts;
+  const int first = part * each + min(part, more);
+  const int ntiles = each + (part < more ? 1 : 0);
+
+  if (warp == DC) {
+    // ---------------- producer ----------------
+    const int32_t* table = a.table + (size_t)b * a.pages_per_seq;
+    bool ok = true;
+    int entry = 0, it = 0;
+    for (; it < ntiles; ++it) {
+      if ((it & 31) == 0) entry = it + lane < ntiles ? __ldcg(table + page_of(seen, first + it + lane)) : 0;
+      const int page = __shfl_sync(0xffffffffu, entry, it & 31);
+      const int s = it % NS;
+      if (it >= NS) {
+        const int landed = mbar_wait(smem_u32(&bars[NS + s]), ((it / NS) - 1) & 1, abort_flag) ? 1 : 0;
+        ok = __all_sync(0xffffffffu, landed);
+        if (!ok) {
+          if (lane == 0) { atomicExch(status, 1); *abort_flag = 1; }
+          break;
+        }
+      }
+      if (lane == 0) {
+        const int at = page_of(seen, first + it), base = at * Q_PAGE_TOKENS;
+        int r0 = 0, r1 = min(Q_PAGE_TOKENS, seen.lim - base);
+        if (at >= seen.sink_pages) r0 = max(0, seen.low - base);
+        else if (seen.low >= base + Q_PAGE_TOKENS) r1 = min(r1, a.sinks - base);
+        const uint32_t bytes = (uint32_t)(r1 - r0) * 256u;
+        const size_t off = ((size_t)page * a.nkv + kh) * ROW_TILE + (size_t)r0 * 256;
+        const uint32_t bar = smem_u32(&bars[s]), dst = smem_u32(stages) + s * ROW_STAGE + r0 * 256;
+        mbar_expect_tx(bar, 2 * bytes);
+        copy_rows(dst, a.kpool + off, bytes, bar);
+        copy_rows(dst + ROW_TILE, a.vpool + off, bytes, bar);
+      }
+      __syncwarp();
+    }
+    // copies in flight land before the CTA may leave, also where a wait ran out
+    if (lane == 0)
+      for (int j = max(0, it - NS); j < it; ++j) mbar_wait_plain(smem_u32(&bars[j % NS]), (j / NS) & 1);
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  } else {
+    // ---------------- consumers ----------------
+    for (int c = tid; c < NT * 8 * 16; c += DC * 32) {
+      const int r = c >> 4, ch = c & 15;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r < R) {
+        const int t = r / a.G, g = r - t * a.G;
+        v = __ldcg(reinterpret_cast<const uint4*>(a.q + ((size_t)(b * a.T + t) * a.nq + kh * a.G + g) * 128) + ch);
+      }
+      *reinterpret_cast<uint4*>(qtile + r * 256 + ((ch ^ (r & 7)) << 4)) = v;
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(DC * 32) : "memory");
+
+    const int g = lane >> 2, t4 = lane & 3;
+    float m_run[NT][2], l_run[NT][2];              // rows 8 n + 2 t4, + 1 (l: of this lane's keys)
+    float oacc[NT][8][4];                          // dims 16 d + g, 16 d + g + 8
+    int lim_r[NT][2], low_r[NT][2];                // what the row sees: [low, lim) and the sinks
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        m_run[n][h] = -INFINITY;
+        l_run[n][h] = 0.f;
+        const int r = 8 * n + 2 * t4 + h, t = r / a.G;
+        lim_r[n][h] = r >= R ? 0 : a.flat ? seen.lim : min(seen.pos + t + 1, seen.lim);
+        low_r[n][h] = a.flat ? 0 : seen.pos + t + 1 - a.window;
+      }
+#pragma unroll
+      for (int d = 0; d < 8; ++d) oacc[n][d][0] = oacc[n][d][1] = oacc[n][d][2] = oacc[n][d][3] = 0.f;
+    }
+    const uint32_t q_base = smem_u32(qtile);
+    uint32_t qf[NT <= 2 ? NT : 1][8][2];           // Q^T fragments; four row tiles read them from shared memory each time
+    if constexpr (NT <= 2) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int kp = 0; kp < 4; ++kp) {
+          const int row = 8 * n + (lane & 7), ch = 4 * kp + (lane >> 3);
+          ldsm_x4(q_base + row * 256 + ((ch ^ (row & 7)) << 4), qf[n][2 * kp][0], qf[n][2 * kp][1],
+                  qf[n][2 * kp + 1][0], qf[n][2 * kp + 1][1]);
+        }
+    }
+    const int grp = warp >> 2, wk = warp & 3;      // tile lane of the warp's group, key quarter of the warp
+    bool ok = true;
+    for (int it = grp; it < ntiles; it += DG) {
+      const int s = it % NS;
+      const int landed = mbar_wait(smem_u32(&bars[s]), (it / NS) & 1, abort_flag) ? 1 : 0;
+      ok = __all_sync(0xffffffffu, landed);
+      if (!ok) {
+        if (lane == 0) { atomicExch(status, 2); *abort_flag = 1; }
+        break;
+      }
+      unsigned char* kt = stages + s * ROW_STAGE;
+      unsigned char* vt = kt + ROW_TILE;
+      const int key0 = page_of(seen, first + it) * Q_PAGE_TOKENS + wk * 16;
+      if (key0 < seen.lim && (key0 + 16 > seen.low || key0 < a.sinks)) {
+        if (key0 + 16 > seen.lim || (key0 < seen.low && key0 + 16 > a.sinks)) {
+          // values that no row sees are cleared: 0 * garbage could be NaN in P V
+          for (int i = lane; i < 16 * 16; i += 32) {
+            const int key = key0 + (i >> 4);
+            if (key >= seen.lim || (key < seen.low && key >= a.sinks))
+              *reinterpret_cast<uint4*>(vt + (wk * 16 + (i >> 4)) * 256 + ((i & 15) << 4)) = make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+        const uint32_t k_base = smem_u32(kt), v_base = smem_u32(vt);
+        float sset[NT][SETS][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int q = 0; q < SETS; ++q) sset[n][q][0] = sset[n][q][1] = sset[n][q][2] = sset[n][q][3] = 0.f;
+        const int arow = wk * 16 + (lane & 7) + 8 * ((lane >> 3) & 1);
+#pragma unroll
+        for (int kp = 0; kp < 4; ++kp) {
+          uint32_t ka[2][4];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int ch = 2 * (2 * kp + e) + (lane >> 4);
+            ldsm_x4(k_base + arow * 256 + ((ch ^ (arow & 7)) << 4), ka[e][0], ka[e][1], ka[e][2], ka[e][3]);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            uint32_t q0, q1, q2, q3;
+            if constexpr (NT <= 2) {
+              q0 = qf[n][2 * kp][0]; q1 = qf[n][2 * kp][1]; q2 = qf[n][2 * kp + 1][0]; q3 = qf[n][2 * kp + 1][1];
+            } else {
+              const int row = 8 * n + (lane & 7), ch = 4 * kp + (lane >> 3);
+              ldsm_x4(q_base + row * 256 + ((ch ^ (row & 7)) << 4), q0, q1, q2, q3);
+            }
+            mma16816(sset[n][(2 * kp) % SETS], ka[0][0], ka[0][1], ka[0][2], ka[0][3], q0, q1);
+            mma16816(sset[n][(2 * kp + 1) % SETS], ka[1][0], ka[1][1], ka[1][2], ka[1][3], q2, q3);
+          }
+        }
+        // every row sees all 16 keys: nothing to mask
+        const bool open = key0 + 16 <= (a.flat ? seen.lim : seen.pos + 1) &&
+                          (a.flat || key0 > seen.pos + a.T - 1 - a.window || key0 + 16 <= a.sinks);
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float sc[4];                           // (key g, row 2 t4), (g, 2 t4 + 1), (g + 8, 2 t4), (g + 8, 2 t4 + 1)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float v = sset[n][0][e];
+            if (SETS == 2) v += sset[n][1][e];
+            if (SETS == 4) v = (v + sset[n][1][e]) + (sset[n][2][e] + sset[n][3][e]);
+            v *= a.scale_log2;
+            if (!open) {
+              const int key = key0 + g + 8 * (e >> 1);
+              v = key < lim_r[n][e & 1] && (key >= low_r[n][e & 1] || key < a.sinks) ? v : -INFINITY;
+            }
+            sc[e] = v;
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float mx = fmaxf(sc[h], sc[2 + h]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float m_new = fmaxf(m_run[n][h], mx);
+            const float m_safe = m_new == -INFINITY ? 0.f : m_new;
+            const float resc = exp2f(m_run[n][h] - m_safe);          // exp2(-inf) = 0 on the first keys
+            sc[h] = exp2f(sc[h] - m_safe);
+            sc[2 + h] = exp2f(sc[2 + h] - m_safe);
+            l_run[n][h] = l_run[n][h] * resc + (sc[h] + sc[2 + h]);
+            m_run[n][h] = m_new;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) { oacc[n][d][h] *= resc; oacc[n][d][2 + h] *= resc; }
+          }
+          pb[n][0] = transpose8x8(pack_bf16(sc[0], sc[1]));
+          pb[n][1] = transpose8x8(pack_bf16(sc[2], sc[3]));
+        }
+        const int mi = lane >> 3, vrow = wk * 16 + 8 * (mi >> 1) + (lane & 7);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          uint32_t v0, v1, v2, v3;
+          const int ch = 2 * d + (mi & 1);
+          ldsm_x4_t(v_base + vrow * 256 + ((ch ^ (vrow & 7)) << 4), v0, v1, v2, v3);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816(oacc[n][d], v0, v1, v2, v3, pb[n][0], pb[n][1]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bars[NS + s]));
+    }
+    // join the consumer warps' states through shared memory (the R real rows), over the ring: every copy has
+    // landed, since every tile was waited for
+    asm volatile("bar.sync 1, %0;" ::"n"(DC * 32) : "memory");
+    float* mo = reinterpret_cast<float*>(stages);            // [DC][R][ROW_LD]
+    float* mml = mo + DC * R * ROW_LD;                       // [DC][R][2]
+    if (*abort_flag == 0) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float l = l_run[n][h];
+          l += __shfl_xor_sync(0xffffffffu, l, 4);
+          l += __shfl_xor_sync(0xffffffffu, l, 8);
+          l += __shfl_xor_sync(0xffffffffu, l, 16);
+          const int r = 8 * n + 2 * t4 + h;
+          if (r < R) {
+            float* dst = mo + (warp * R + r) * ROW_LD + g;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) { dst[16 * d] = oacc[n][d][h]; dst[16 * d + 8] = oacc[n][d][2 + h]; }
+            if (g == 0) {
+              mml[(warp * R + r) * 2] = m_run[n][h];
+              mml[(warp * R + r) * 2 + 1] = l;
+            }
+          }
+        }
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(DC * 32) : "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    const int d = tid & 127;
+    for (int r = tid >> 7; r < R && *abort_flag == 0; r += DG) {
+      float mw[DC], Mx = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < DC; ++w) { mw[w] = mml[(w * R + r) * 2]; Mx = fmaxf(Mx, mw[w]); }
+      const float Ms = Mx == -INFINITY ? 0.f : Mx;
+      float Lsum = 0.f, O = 0.f;
+#pragma unroll
+      for (int w = 0; w < DC; ++w) {
+        const float wt = exp2f(mw[w] - Ms);
+        Lsum += wt * mml[(w * R + r) * 2 + 1];
+        O += wt * mo[(w * R + r) * ROW_LD + d];
+      }
+      // to the CTA that joins this (row, dim): slot `rank` of its receive area
+      const int v = r * 128 + d, owner = v / a.share;
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote_addr(smem_u32(recv), owner) +
+                   (uint32_t)(rank * a.share + (v - owner * a.share)) * 4u), "f"(O) : "memory");
+      if (d < S)           // the row's maximum and sum go to every CTA of the cluster (thread d -> CTA d)
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(remote_addr(smem_u32(recv), d) +
+                     (uint32_t)(S * a.share + (rank * R + r) * 2) * 4u), "f"(Mx), "f"(Lsum) : "memory");
+    }
+  }
+  // everything this CTA joins is in its own memory behind the barrier: no remote reads, and no second
+  // barrier before it may leave
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (a.early) pdl_wait();       // the prefix's partial rows are complete
+  const float* rml = recv + S * a.share;
+  const int total = R * 128, own0 = rank * a.share;
+  const int psplits = a.parts.splits > 0 && !a.write_parts ? parts_used(a.parts) : 0;
+  for (int c = warp * 32; c < a.share && own0 + c < total; c += DT) {
+    const int r = (own0 + c) >> 7, d = ((own0 + c) & 127) + lane;
+    const int t = r / a.G, hg = r - t * a.G;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < S) ml = *reinterpret_cast<const float2*>(rml + (lane * R + r) * 2);
+    // the prefix's parts of this row: lane and lane + 32
+    float2 pml[2] = {make_float2(-INFINITY, 0.f), make_float2(-INFINITY, 0.f)};
+    const size_t prow = (size_t)(b * a.T + t) * a.G + hg;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (lane + 32 * e < psplits) pml[e] = __ldcg(a.parts.ml + a.parts.row(lane + 32 * e, kh, prow));
+    float Mx = warp_max(fmaxf(ml.y > 0.f ? ml.x : -INFINITY,
+                              fmaxf(pml[0].y > 0.f ? pml[0].x : -INFINITY, pml[1].y > 0.f ? pml[1].x : -INFINITY)));
+    if (Mx == -INFINITY) Mx = 0.f;
+    const float w = ml.y > 0.f ? exp2f(ml.x - Mx) : 0.f;
+    const float pw[2] = {pml[0].y > 0.f ? exp2f(pml[0].x - Mx) : 0.f, pml[1].y > 0.f ? exp2f(pml[1].x - Mx) : 0.f};
+    // NaN (a NaN among the visible keys) is carried on
+    float l = (ml.y == ml.y ? w * ml.y : ml.y) + (pml[0].y == pml[0].y ? pw[0] * pml[0].y : pml[0].y) +
+              (pml[1].y == pml[1].y ? pw[1] * pml[1].y : pml[1].y);
+    l = warp_sum(l);
+    float O = 0.f;
+    for (int s = 0; s < S; ++s) O += __shfl_sync(0xffffffffu, w, s) * recv[s * a.share + c + lane];
+    for (int s0 = 0; s0 < psplits; s0 += 8) {
+      float o[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        o[j] = s0 + j < psplits ? __ldcg(a.parts.o + a.parts.row(s0 + j, kh, prow) * 128 + d) : 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float lo = __shfl_sync(0xffffffffu, pw[0], (s0 + j) & 31), hi = __shfl_sync(0xffffffffu, pw[1], (s0 + j) & 31);
+        O += (s0 + j < 32 ? lo : hi) * o[j];
+      }
+    }
+    if (a.write_parts) {
+      const size_t row = a.parts.row(blockIdx.x / S, kh, prow);
+      a.parts.o[row * 128 + d] = O;
+      if (d == 0) a.parts.ml[row] = make_float2(Mx, l);
+    } else {
+      const float res = l > 0.f ? O / l : l == 0.f ? 0.f : l;
+      a.out[((size_t)(b * a.T + t) * a.nq + kh * a.G + hg) * 128 + d] = __float2bfloat16_rn(res);
+    }
+  }
+}
+
+// How a launch splits: CTAs of a cluster, clusters of a (sequence, kv head), warp groups, ring stages.
+struct RowsPlan { int nt, groups, splits, clusters, stages, share; size_t smem; };
+
+// vh: (sequence, kv head) pairs; pages: most pages a pair's rows can see. join: the splits merge in one
+// cluster; otherwise the pages go to as many clusters as fill the SMs.
+RowsPlan rows_plan(int vh, int rows, long long pages, bool join) {
+  RowsPlan p;
+  p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  int sms = q_sm_count();
+  if (sms <= 0) sms = 148;
+  auto least = [](long long a, long long b) { return (int)(a < b ? a : b); };
+  p.clusters = 1;
+  p.groups = p.nt == 4 ? 2 : 1;
+  const int per_sm = p.nt == 4 ? 1 : 2;
+  p.splits = least(least(MAX_SPLITS, pages), (long long)per_sm * sms / vh);
+  if (p.nt == 1) {
+    // every CTA an SM of its own, three groups of warps: the tiles of a split side by side
+    const int wide = least(least(MAX_SPLITS, (pages - 1) / 2), sms / vh);
+    if (wide >= 2) { p.groups = 3; p.splits = wide; }
+  }
+  if (p.splits < 1) p.splits = 1;
+  if (!join) {
+    p.clusters = least(pages / p.splits, (long long)(p.groups == 1 ? per_sm : 1) * sms / ((long long)vh * p.splits));
+    if (p.clusters < 1) p.clusters = 1;
+    if (p.clusters > 64) p.clusters = 64;
+  }
+  const long long each = (pages + (long long)p.splits * p.clusters - 1) / ((long long)p.splits * p.clusters);
+  const int dc = 4 * p.groups;
+  p.stages = p.nt == 4 ? 6 : 3;
+  const int need = (dc * rows * (ROW_LD + 2) * 4 + ROW_STAGE - 1) / ROW_STAGE;       // the warps' states lie over the ring
+  if (each < p.stages) p.stages = (int)each;
+  // a stage always belongs to the same group of warps, which tracks its parity
+  if (p.groups == 3) p.stages = 3;
+  if (p.groups == 2) p.stages += p.stages & 1;
+  if (p.stages < need) p.stages = need;
+  if (p.groups == 2) p.stages += p.stages & 1;
+  p.share = ((rows * 128 + p.splits - 1) / p.splits + 31) / 32 * 32;
+  p.smem = (size_t)p.stages * ROW_STAGE + p.nt * 8 * 256 + 16 * p.stages + 16 + (size_t)(p.splits * p.share + p.splits * rows * 2) * 4;
+  return p;
+}
+
+template <int NT, int DG>
+cudaError_t rows_go(const RowsPlan& p, const RowsArgs& a, int vh, int* status, cudaStream_t stream) {
+  static size_t done[64] = {0};
+  cudaError_t e = q_ensure_smem(k_attn_rows<NT, DG>, p.smem, done);
+  if (e != cudaSuccess) return e;
+  return q_launch_cluster(k_attn_rows<NT, DG>, dim3(p.splits * p.clusters, vh), dim3((4 * DG + 1) * 32), p.smem, stream,
+                          (unsigned)p.splits, a, status);
+}
+
+int rows_launch(const RowsPlan& p, RowsArgs& a, int vh, const char* who, cudaStream_t stream) {
+  int* status = q_attn_status_addr();
+  if (!status) { q_set_error("%s: could not locate the device status word", who); return Q_ERR_CUDA; }
+  a.share = p.share;
+  a.stages = p.stages;
+  if (p.nt == 4) Q_CHECK_CUDA((rows_go<4, 2>(p, a, vh, status, stream)));
+  else if (p.nt == 2) Q_CHECK_CUDA((rows_go<2, 1>(p, a, vh, status, stream)));
+  else if (p.groups == 3) Q_CHECK_CUDA((rows_go<1, 3>(p, a, vh, status, stream)));
+  else Q_CHECK_CUDA((rows_go<1, 1>(p, a, vh, status, stream)));
+  return Q_OK;
+}
+
+int check_rows(const char* who, const void* d_q, const q_kv_layout_t* kv, const int32_t* d_pos, const void* d_out,
+               int batch, int T, int n_q_heads) {
+  Q_CHECK_ARG(d_q && kv && d_pos && d_out, "%s: null pointer", who);
+  Q_CHECK_ARG(kv->d_kpool && kv->d_vpool && kv->d_block_table && kv->pages_per_seq >= 1 && kv->n_kv_heads >= 1,
+              "%s: incomplete KV layout", who);
+  const int nkv = kv->n_kv_heads;
+  Q_CHECK_ARG(batch >= 1 && T >= 1 && n_q_heads >= nkv && n_q_heads % nkv == 0, "%s: bad batch/T/heads", who);
+  const int G = n_q_heads / nkv;
+  Q_CHECK_ARG((long long)T * G <= 32, "%s: T*G = %lld exceeds 32 query rows per kv head", who, (long long)T * G);
+  Q_CHECK_ARG((long long)batch * nkv <= 65535, "%s: too many (sequence, kv head) pairs", who);
+  Q_CHECK_ARG(kv->pages_per_seq <= (1 << 24), "%s: too many pages per sequence", who);
+  Q_CHECK_ALIGN(d_q, 16, who); Q_CHECK_ALIGN(kv->d_kpool, 16, who); Q_CHECK_ALIGN(kv->d_vpool, 16, who);
+  Q_CHECK_ALIGN(d_out, 2, who); Q_CHECK_ALIGN(d_pos, 4, who); Q_CHECK_ALIGN(kv->d_block_table, 4, who);
+  return Q_OK;
+}
+
+RowsArgs rows_args(const void* d_q, const q_kv_layout_t* kv, const int32_t* d_pos, int pos_per_seq, void* d_out,
+                   int T, int n_q_heads, float scale) {
+  RowsArgs a = {};
+  a.q = (const bf16*)d_q;
+  a.kpool = (const char*)kv->d_kpool;
+  a.vpool = (const char*)kv->d_vpool;
+  a.table = kv->d_block_table;
+  a.pos = d_pos;
+  a.pos_step = pos_per_seq ? 1 : 0;
+  a.out = (bf16*)d_out;
+  a.pages_per_seq = kv->pages_per_seq;
+  a.nkv = kv->n_kv_heads;
+  a.nq = n_q_heads;
+  a.T = T;
+  a.G = n_q_heads / kv->n_kv_heads;
+  a.window = 1 << 30;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  return a;
+}
+
+}  // namespace
+
+extern "C" int q_attention_window(const void* d_q, const q_kv_layout_t* kv, const int32_t* d_pos, int pos_per_seq,
+                                  void* d_out, int batch, int T, int n_q_heads, int window, int sinks, float scale,
+                                  void* stream) {
+  const char* who = "q_attention_window";
+  const int rc = check_rows(who, d_q, kv, d_pos, d_out, batch, T, n_q_heads);
+  if (rc) return rc;
+  Q_CHECK_ARG(window >= 1 && sinks >= 0, "%s: window %d / sinks %d", who, window, sinks);
+  RowsArgs a = rows_args(d_q, kv, d_pos, pos_per_seq, d_out, T, n_q_heads, scale);
+  a.window = window < (1 << 30) ? window : 1 << 30;
+  a.sinks = sinks < (1 << 30) ? sinks : 1 << 30;
+  // most pages a sequence's rows can see: those of window + T - 1 consecutive keys, and the sinks'
+  const long long all = kv->pages_per_seq;
+  long long pages = ((long long)a.window + T - 2) / Q_PAGE_TOKENS + 2 + ((long long)a.sinks + Q_PAGE_TOKENS - 1) / Q_PAGE_TOKENS;
+  if (pages > all) pages = all;
+  const RowsPlan p = rows_plan(batch * kv->n_kv_heads, T * a.G, pages, true);
+  return rows_launch(p, a, batch * kv->n_kv_heads, who, (cudaStream_t)stream);
+}

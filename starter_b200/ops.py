@@ -223,15 +223,31 @@ class PagedKV:
     """
 
     def __init__(self, batch: int, n_kv_heads: int, capacity: int, device,
-                 block_table: torch.Tensor | None = None, poison: float | None = None):
+                 block_table: torch.Tensor | None = None, poison: float | None = None,
+                 pools: tuple[torch.Tensor, torch.Tensor] | None = None):
+        """pools: the (K, V) pages to use instead of own ones, [pages, n_kv_heads, 64, 128] each (an engine's layer,
+        or pages that several caches share, each through a block table of its own)."""
         if min(batch, n_kv_heads, capacity) < 1:
             raise ValueError("positive batch, head count and capacity required")
         self.batch, self.n_kv, self.capacity = batch, n_kv_heads, capacity
         self.pages_per_seq = (capacity + PAGE_TOKENS - 1) // PAGE_TOKENS
         n_pages = batch * self.pages_per_seq
-        shape = (n_pages, n_kv_heads, PAGE_TOKENS, HEAD_DIM)
-        self.k = torch.zeros(shape, dtype=torch.bfloat16, device=device)
-        self.v = torch.zeros(shape, dtype=torch.bfloat16, device=device)
+        if pools is not None:
+            self.k, self.v = pools
+            if (self.k.ndim != 4 or self.k.shape != self.v.shape
+                    or tuple(self.k.shape[1:]) != (n_kv_heads, PAGE_TOKENS, HEAD_DIM)
+                    or any(p.dtype != torch.bfloat16 or not p.is_contiguous() or p.device != self.k.device
+                           for p in pools)):
+                raise ValueError("pools must be two contiguous BF16 [pages, n_kv_heads, 64, 128] tensors of one device")
+            if block_table is None and self.k.shape[0] < n_pages:
+                raise ValueError("the pools have fewer pages than the sequences")
+            if poison is not None:
+                raise ValueError("poison fills new pools only")
+            device = self.k.device
+        else:
+            shape = (n_pages, n_kv_heads, PAGE_TOKENS, HEAD_DIM)
+            self.k = torch.zeros(shape, dtype=torch.bfloat16, device=device)
+            self.v = torch.zeros(shape, dtype=torch.bfloat16, device=device)
         if poison is not None:
             self.k.fill_(poison)
             self.v.fill_(poison)
@@ -364,6 +380,55 @@ def prompt_attention(query: torch.Tensor, cache: PagedKV, position: torch.Tensor
     check(lib.q_attention_prefill(_ptr(query), C.byref(cache.layout), _ptr(position), _ptr(out), cache.batch,
                                   T, hq, float(scale), _stream()))
     return out
+
+
+def _positions(position: torch.Tensor, batch: int, device) -> int:
+    """Checks an int32 CUDA position tensor of shape [1] (all sequences) or [batch]; whether it has one per
+    sequence."""
+    if (tuple(position.shape) not in ((1,), (batch,)) or position.dtype != torch.int32 or position.device != device
+            or not position.is_contiguous()):
+        raise ValueError("position must be a contiguous int32 tensor of shape [1] or [batch] on the query's device")
+    return int(position.shape[0] == batch)
+
+
+def _paged_query(query: torch.Tensor, cache: PagedKV, rows: int, heads: int | None) -> None:
+    if (query.ndim != 3 or query.shape[0] != rows or query.shape[2] != HEAD_DIM
+            or (heads is not None and query.shape[1] != heads)
+            or query.dtype != torch.bfloat16 or not query.is_cuda or not query.is_contiguous()):
+        raise ValueError("expected contiguous BF16 CUDA Q [batch*T, Hq, 128]")
+    if cache.k.device != query.device or cache.block_table.device != query.device:
+        raise ValueError("query and cache are on different devices")
+
+
+class WindowAttention:
+    """GQA attention of 1..32/G query tokens per sequence under a sliding window with sinks: SmallQueryAttention
+    whose row (b, t, head), at p = position + t, attends to the keys j <= p with j > p - window or j < sinks.
+
+    position is int32 [1] for all sequences or [batch]. Pages that hold no visible key are not read, so that a
+    server may reuse them while the sequence lives; keys keep the rotation they were stored with. No scratch: calls
+    may run on any streams."""
+
+    def __init__(self, batch, query_heads, kv_heads, capacity, device, window, sinks=0, tokens_per_seq=1):
+        device = torch.device(device)
+        if (device.type != "cuda" or min(batch, query_heads, kv_heads, capacity, tokens_per_seq) < 1
+                or query_heads % kv_heads or tokens_per_seq * (query_heads // kv_heads) > 32):
+            raise ValueError("unsupported small-query attention metadata")
+        if not 1 <= window < 2 ** 31 or not 0 <= sinks < 2 ** 31:
+            raise ValueError("the window must hold at least one key, and sinks cannot be negative")
+        self.batch, self.hq, self.hk, self.capacity = batch, query_heads, kv_heads, capacity
+        self.T, self.window, self.sinks = tokens_per_seq, int(window), int(sinks)
+
+    def run(self, query, cache: PagedKV, position, scale) -> torch.Tensor:
+        """query [batch*T, Hq, 128] -> [batch*T, Hq*128]."""
+        _paged_query(query, cache, self.batch * self.T, self.hq)
+        if cache.batch != self.batch or cache.n_kv != self.hk or cache.capacity < self.capacity:
+            raise ValueError("cache does not match this attention instance")
+        each = _positions(position, self.batch, query.device)
+        with torch.cuda.device(query.device):
+            out = torch.empty((self.batch * self.T, self.hq * HEAD_DIM), dtype=torch.bfloat16, device=query.device)
+            check(lib.q_attention_window(_ptr(query), C.byref(cache.layout), _ptr(position), each, _ptr(out),
+                                         self.batch, self.T, self.hq, self.window, self.sinks, float(scale), _stream()))
+        return out
 
 
 def decode_attention(qkv, q_weight, k_weight, eps, cos, sin, position, cache: PagedKV,

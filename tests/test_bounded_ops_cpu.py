@@ -1,0 +1,69 @@
+"""Refusals of the windowed, shared-prefix and sampling operators: all on the host, before any launch."""
+import ctypes as C
+
+import pytest
+import torch
+
+A = 4096          # a made-up, aligned address: nothing is launched
+
+
+def layout(nkv=2, pages=3, k=A, v=A, table=A):
+    from starter_b200._lib import KVLayout
+    return KVLayout(k, v, table, pages, nkv)
+
+
+def refused(rc, text=None):
+    from starter_b200 import _lib
+    message = (_lib.lib.q_last_error() or b"").decode()
+    assert rc == -1, message
+    if text:
+        assert text in message, message
+
+
+def test_window_attention_refuses_bad_arguments():
+    from starter_b200._lib import lib
+    kv = layout()
+
+    def call(q=A, kv=kv, pos=A, out=A, batch=1, T=1, nq=8, window=5, sinks=0):
+        return lib.q_attention_window(q, C.byref(kv) if kv else None, pos, 0, out, batch, T, nq, window, sinks, 0.1, None)
+    refused(call(q=None), "null")
+    refused(call(kv=None), "null")
+    refused(call(pos=None), "null")
+    refused(call(out=None), "null")
+    refused(call(q=A + 8), "aligned")
+    refused(call(kv=layout(k=A + 8)), "aligned")
+    refused(call(pos=A + 2), "aligned")
+    refused(call(kv=layout(pages=0)), "incomplete")
+    refused(call(batch=0))
+    refused(call(T=0))
+    refused(call(nq=7))
+    refused(call(nq=2, T=33), "32 query rows")
+    refused(call(window=0), "window")
+    refused(call(sinks=-1), "sinks")
+    refused(call(batch=40000), "too many")
+
+
+def test_window_attention_class_refuses_before_a_launch():
+    from starter_b200 import ops
+    for bad in (dict(window=0), dict(window=5, sinks=-1), dict(window=5, tokens_per_seq=9), dict(window=2 ** 31)):
+        with pytest.raises(ValueError):
+            ops.WindowAttention(1, 32, 8, 100, "cuda", **bad)
+    with pytest.raises(ValueError):
+        ops.WindowAttention(1, 32, 8, 100, "cpu", 5)
+    attn = ops.WindowAttention(1, 8, 2, 100, "cuda", 5)
+    cache = ops.PagedKV(1, 2, 100, "cpu")
+    with pytest.raises(ValueError):
+        attn.run(torch.zeros((1, 8, 128), dtype=torch.bfloat16), cache, torch.zeros(1, dtype=torch.int32), 0.1)
+
+
+def test_caches_over_given_pages():
+    from starter_b200 import ops
+    k, v = (torch.zeros((6, 2, 64, 128), dtype=torch.bfloat16) for _ in range(2))
+    cache = ops.PagedKV(2, 2, 150, "cpu", pools=(k, v))
+    assert cache.k is k and cache.v is v and cache.layout.d_kpool == k.data_ptr()
+    table = torch.tensor([[5, 0]], dtype=torch.int32)
+    assert ops.PagedKV(1, 2, 100, "cpu", block_table=table, pools=(k, v)).block_table is table
+    for bad in (dict(pools=(k[:5], v[:5])), dict(pools=(k, v[:5])), dict(pools=(k.float(), v.float())),
+                dict(pools=(k, v), poison=1.0), dict(pools=(k[:, :1], v[:, :1]))):
+        with pytest.raises(ValueError):
+            ops.PagedKV(2, 2, 150, "cpu", **bad)
