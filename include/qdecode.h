@@ -366,6 +366,23 @@ int q_attention_window(const void* d_q, const q_kv_layout_t* kv, const int32_t* 
                        void* d_out, int batch, int T, int n_q_heads, int window, int sinks, float scale,
                        void* stream);
 
+/* q_attention_prefill under the same window: row (b, t, head) of T prompt tokens, any T, up to 32 query heads per kv
+ * head. Positions are not negative; d_out 4-byte aligned. */
+int q_attention_window_prefill(const void* d_q, const q_kv_layout_t* kv, const int32_t* d_pos, int pos_per_seq,
+                               void* d_out, int batch, int T, int n_q_heads, int window, int sinks, float scale,
+                               void* stream);
+
+/* Attention of a batch that shares a prefix: row (b, t, head) attends to keys [0, *d_prefix_len) of the one
+ * sequence in `prefix`, read once for the whole batch, and to keys [0, pos + t] of sequence b in `kv` (which may lie
+ * in the same pools). Two launches: the prefix in key splits that leave partial results in d_scratch
+ * (q_attention_shared_scratch_bytes(), 16-byte aligned; one call at a time may use it), then the sequences' own keys, joined
+ * with them. T * n_q / n_kv <= 32. A prefix length beyond the prefix's pages is cut to them; a row
+ * that sees no key gives zeros. 0 bytes: sizes that q_attention_shared refuses. */
+int64_t q_attention_shared_scratch_bytes(int batch, int T, int n_q_heads, int n_kv_heads, int prefix_pages);
+int q_attention_shared(const void* d_q, const q_kv_layout_t* prefix, const int32_t* d_prefix_len,
+                       const q_kv_layout_t* kv, const int32_t* d_pos, int pos_per_seq, void* d_scratch,
+                       void* d_out, int batch, int T, int n_q_heads, float scale, void* stream);
+
 /* The three kernels above for the single-token decode step in ONE launch:
  * engine/kernels/decode_fused.py:172-210 (head norm + RoPE + K/V write into the page
  * slot *d_pos) + engine/kernels/small_query_attention.py:113-158 (split-KV attention and

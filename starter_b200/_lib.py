@@ -149,6 +149,9 @@ SIGNATURES = {
     "q_attention": (_I, [_P, _KV, _P, _P, _P, _P, _I, _I, _I, _I, _F, _P]),
     "q_attention_prefill": (_I, [_P, _KV, _P, _P, _I, _I, _I, _F, _P]),
     "q_attention_window": (_I, [_P, _KV, _P, _I, _P, _I, _I, _I, _I, _I, _F, _P]),
+    "q_attention_window_prefill": (_I, [_P, _KV, _P, _I, _P, _I, _I, _I, _I, _I, _F, _P]),
+    "q_attention_shared_scratch_bytes": (C.c_int64, [_I, _I, _I, _I, _I]),
+    "q_attention_shared": (_I, [_P, _KV, _P, _KV, _P, _I, _P, _P, _I, _I, _I, _F, _P]),
     "q_attention_decode": (_I, [_P, _PLAN, _P, _P, _P, _P, _P, _KV, _P, _P, _P, _P, _I, _I, _I, _F, _F, _P]),
     "q_argmax_scratch_bytes": (C.c_int64, [_I, _I]),
     "q_logits_argmax": (_I, [_P, _PLAN, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P]),

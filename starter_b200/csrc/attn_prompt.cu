@@ -29,7 +29,14 @@
 // Tiles are read through tensor maps whose boxes undo the 256-byte row pitch of a page: a box of
 // 64 rows x 64 dims lands as rows of 128 bytes, and the pages' own chunk swizzle (chunk ^ row & 7)
 // is then the 128-byte swizzle the MMA descriptors name. Every wait is bounded.
+//
+// Three forms (FORM) walk other keys with the same pipeline: CAUSAL (the prompt), WINDOW (the prompt under a
+// sliding window with sinks: of the key tiles only those that hold a key some row of the item sees), PARTS (many
+// rows over one range of keys that all of them see, cut into key splits whose m, l and O are left in 32 bits).
+// In the last two any head count per kv head up to 128 is taken, k steps of 16 keys that nobody sees are left out
+// of P V, and of a tile that nobody sees in one of its pages that page is not read.
 #include "tc.cuh"
+#include "attn_parts.cuh"
 
 int* q_attn_status_addr();
 
@@ -54,9 +61,18 @@ struct AttnShape {
   int items;
   int wide;          // the output is 32-byte aligned
   float scale_log2;
+  int pos_step, window, sinks, room;     // WINDOW: positions per sequence, keys that the table's pages hold (PARTS: too)
+  AttnParts parts;                       // PARTS
 };
 
-struct Item { int b, kh, q0, n, max_limit; };
+enum Form { CAUSAL, WINDOW, PARTS };
+
+struct Item {
+  int b, kh, q0, n, max_limit;
+  int pos, low;                          // WINDOW: position of token 0, oldest key of the item's first window
+  int sink_tiles, skip;                  // tile j is key tile j, + skip from sink_tiles on (PARTS: sink_tiles 0)
+  int split;
+};
 
 __device__ __forceinline__ Item item_at(const AttnShape& sh, int w, int pos) {
   Item it;
@@ -68,6 +84,60 @@ __device__ __forceinline__ Item item_at(const AttnShape& sh, int w, int pos) {
   it.max_limit = pos + min(it.q0 + sh.tiles * sh.tokens, sh.T);
   it.n = (it.max_limit + AP_KEYS - 1) / AP_KEYS;
   return it;
+}
+// `pos`: the position (CAUSAL), the number of keys (PARTS), nothing (WINDOW, where every sequence has its own).
+template <int FORM>
+__device__ __forceinline__ Item item_of_form(const AttnShape& sh, int w, int pos, const int32_t* pos_ptr) {
+  if constexpr (FORM == CAUSAL) return item_at(sh, w, pos);
+  Item it;
+  if constexpr (FORM == WINDOW) {
+    const int heads = sh.batch * sh.nkv;
+    const int blk = w / heads, bh = w - blk * heads;
+    it.b = bh / sh.nkv;
+    it.kh = bh - it.b * sh.nkv;
+    it.q0 = (sh.blocks - 1 - blk) * sh.tiles * sh.tokens;
+    // positions outside the pages read nothing outside the table
+    it.pos = min(max(__ldcg(pos_ptr + (size_t)it.b * sh.pos_step), 0), sh.room - 1);
+    it.max_limit = min(it.pos + min(it.q0 + sh.tiles * sh.tokens, sh.T), sh.room);
+    it.low = min(max(0, it.pos + it.q0 - sh.window + 1), it.max_limit - 1);
+    it.sink_tiles = (min(sh.sinks, it.max_limit) + AP_KEYS - 1) / AP_KEYS;
+    const int first = max(it.sink_tiles, it.low / AP_KEYS);
+    it.skip = first - it.sink_tiles;
+    it.n = it.sink_tiles + max(0, (it.max_limit + AP_KEYS - 1) / AP_KEYS - first);
+    it.split = 0;
+  } else {
+    // query blocks of a (split, kv head) next to one another: they share its keys in L2
+    const int blk = w % sh.blocks, sk = w / sh.blocks;
+    it.b = 0;
+    it.split = sk / sh.nkv;
+    it.kh = sk - it.split * sh.nkv;
+    it.q0 = blk * sh.tiles * sh.tokens;
+    it.max_limit = pos;
+    it.pos = it.low = it.sink_tiles = 0;
+    const int tiles = (pos + AP_KEYS - 1) / AP_KEYS, splits = min(sh.parts.splits, tiles);
+    const int each = tiles / splits, more = tiles - each * splits;
+    it.skip = it.split * each + min(it.split, more);
+    it.n = each + (it.split < more ? 1 : 0);
+  }
+  return it;
+}
+// First key of an item's tile j.
+template <int FORM>
+__device__ __forceinline__ int key_base_of(const Item& it, int j) {
+  if constexpr (FORM == CAUSAL) return j * AP_KEYS;
+  return (j + (j >= it.sink_tiles ? it.skip : 0)) * AP_KEYS;
+}
+// The k steps (16 keys each) of a tile in which some row of the item sees a key.
+template <int FORM>
+__device__ __forceinline__ uint32_t live_steps(const AttnShape& sh, const Item& it, int key_base) {
+  const int hi = min(AP_KEYS, it.max_limit - key_base);
+  uint32_t live = (1u << ((hi + 15) >> 4)) - 1u;
+  if (FORM == WINDOW && it.low > key_base) {
+    const uint32_t near = 0xffu << (min(it.low - key_base, AP_KEYS) >> 4);
+    const uint32_t far = (1u << ((min(max(sh.sinks - key_base, 0), AP_KEYS) + 15) >> 4)) - 1u;
+    live &= near | far;
+  }
+  return live & 0xffu;
 }
 // The items of a CTA: rounds of gridDim.x, every other round backwards, so that the lengths (which
 // fall with the item number) even out.
@@ -155,7 +225,7 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-template <int TILES>
+template <int TILES, int FORM>
 __global__ void __launch_bounds__(AP_THREADS, 1)
 k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
               const __grid_constant__ CUtensorMap vmap, const int32_t* __restrict__ block_table,
@@ -171,7 +241,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   auto bar = [&](int kind, int i) { return bars + 8u * (uint32_t)(kind + i); };
 
-  pdl_launch_dependents();
+  if (FORM == CAUSAL) pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < 24; ++i) {
@@ -201,9 +271,18 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
   // one may write those. All are requested at once, behind the wait: reading position and pages before
   // it, as the decode kernel does, gained 1 us in a prompt of 64 tokens (12 layers, 1128.7 / 1129.6 us).
   pdl_wait();
-  const int pos = *reinterpret_cast<const volatile int32_t*>(pos_ptr);
+  // (the other forms' dependents may read early whatever the launches before this one wrote)
+  if (FORM != CAUSAL) pdl_launch_dependents();
+  int pos = FORM == WINDOW ? 0 : *reinterpret_cast<const volatile int32_t*>(pos_ptr);
+  int items = sh.items;
+  if (FORM == PARTS) {
+    pos = min(max(pos, 0), sh.room);
+    items = min(sh.parts.splits, (pos + AP_KEYS - 1) / AP_KEYS) * sh.nkv * sh.blocks;
+  }
+  // with fewer tiles than splits some CTAs have no item
+  const bool idle = FORM == PARTS && item_of(0) >= items;
   int first_page[2] = {0, 0};
-  if (warp == 16) {                                        // the grid has at most one CTA per item
+  if (FORM == CAUSAL && warp == 16) {                      // the grid has at most one CTA per item
     const volatile int32_t* table = block_table + (size_t)item_at(sh, item_of(0), 0).b * sh.pages_per_seq;
     first_page[0] = table[0];
     first_page[1] = table[min(1, sh.pages_per_seq - 1)];
@@ -216,14 +295,14 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
       uint32_t nitems = 0;
       bool ok = true;
       auto fail = [&]() { atomicExch(status, 7); *abort_flag = 1; ok = false; };
-      for (int r = 0; ok && r * (int)gridDim.x < sh.items; ++r) {
+      for (int r = 0; ok && r * (int)gridDim.x < items; ++r) {
         const int w = item_of(r);
-        if (w >= sh.items) continue;
-        const Item it = item_at(sh, w, pos);
+        if (w >= items) continue;
+        const Item it = item_of_form<FORM>(sh, w, pos, pos_ptr);
         for (int i = 0; ok && i < TILES; ++i) {
           if (!mbar_wait(bar(B_QE, i), (nitems & 1) ^ 1, abort_flag)) { fail(); break; }
           const int tok = it.b * sh.T + it.q0 + i * sh.tokens;
-          mbar_expect_tx(bar(B_QF, i), AP_TILE);
+          mbar_expect_tx(bar(B_QF, i), FORM == CAUSAL ? AP_TILE : (uint32_t)(sh.tokens * sh.G) * 256u);
           for (int h = 0; h < 2; ++h)
             tma_load_3d(base + AP_Q + i * AP_TILE + h * AP_HALF, &qmap, 64 * h, it.kh * sh.G, tok, bar(B_QF, i));
         }
@@ -232,15 +311,24 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
         for (int j = 0; ok && j < it.n; ++j, ++step) {
           const int s = step & 1;
           const uint32_t parity = ((step >> 1) & 1) ^ 1;
-          const int np = min(2, npages - 2 * j);
-          const int page0 = step ? table[2 * j] : first_page[0];
-          const int page1 = np < 2 ? 0 : step ? table[2 * j + 1] : first_page[1];
+          int np = min(2, npages - 2 * j), page0, page1, p0 = 0;
+          if constexpr (FORM == CAUSAL) {
+            page0 = step ? table[2 * j] : first_page[0];
+            page1 = np < 2 ? 0 : step ? table[2 * j + 1] : first_page[1];
+          } else {
+            const int key_base = key_base_of<FORM>(it, j), at = key_base / Q_PAGE_TOKENS;
+            const uint32_t live = live_steps<FORM>(sh, it, key_base);
+            p0 = live & 0x0fu ? 0 : 1;                     // a page that nobody sees is not read, nor its table entry
+            np = live & 0xf0u ? 2 : 1;
+            page0 = p0 == 0 ? __ldcg(table + at) : 0;
+            page1 = np == 2 ? __ldcg(table + at + 1) : 0;
+          }
           for (int kv = 0; kv < 2; ++kv) {
             if (!mbar_wait(bar(kv ? B_VE : B_KE, s), parity, abort_flag)) { fail(); break; }
             const uint32_t full = bar(kv ? B_VF : B_KF, s);
             const uint32_t dst = base + (kv ? AP_V : AP_K) + s * AP_TILE;
-            mbar_expect_tx(full, (uint32_t)np * AP_HALF);
-            for (int p = 0; p < np; ++p)
+            mbar_expect_tx(full, (uint32_t)(np - p0) * AP_HALF);
+            for (int p = p0; p < np; ++p)
               for (int h = 0; h < 2; ++h)
                 tma_load_4d(dst + h * AP_HALF + p * (AP_HALF / 2), kv ? &vmap : &kmap, 0, h, 0,
                             (p ? page1 : page0) * sh.nkv + it.kh, full);
@@ -293,7 +381,8 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
         tc_commit(bar(B_SF, i));
       };
       int r = 0;
-      Item cur = item_at(sh, item_of(0), pos);             // the grid has at most one CTA per item
+      if (idle) ok = false;                                // (nothing is waited for)
+      Item cur = item_of_form<FORM>(sh, idle ? 0 : item_of(0), idle ? 1 : pos, pos_ptr);  // the grid has at most one CTA per item
       for (int i = 0; i < TILES && ok; ++i) {
         if (!wait(bar(B_QF, i), 0) || (i == 0 && !wait(bar(B_KF, 0), 0))) break;
         scores(i);
@@ -308,9 +397,9 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
         // the item after this one
         bool more = false;
         Item nxt = cur;
-        for (++r; r * (int)gridDim.x < sh.items; ++r) {
+        for (++r; r * (int)gridDim.x < items; ++r) {
           const int w = item_of(r);
-          if (w < sh.items) { nxt = item_at(sh, w, pos); more = true; break; }
+          if (w < items) { nxt = item_of_form<FORM>(sh, w, pos, pos_ptr); more = true; break; }
         }
         for (int j = 0; ok && j < cur.n; ++j) {
           const bool last = j + 1 == cur.n, ahead = !last || more;
@@ -320,9 +409,20 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
             if (j == 0 && !wait(bar(B_OE, i), (nitems & 1) ^ 1)) break;
             // P comes in two halves of 64 keys, from different warps
             if (!wait(bar(B_P, 2 * i), vstep & 1) || !wait(bar(B_P, 2 * i + 1), vstep & 1)) break;
-            const int keys = cur.max_limit - j * AP_KEYS;      // in the last tile, k steps past the newest key are left out
+            const int keys = cur.max_limit - key_base_of<FORM>(cur, j);  // in the last tile, k steps past the newest key are left out
+            uint32_t live = 0;
+            if (FORM == WINDOW) live = live_steps<FORM>(sh, cur, key_base_of<FORM>(cur, j));
             if (elect_one()) {
-              if (keys >= AP_KEYS) {
+              if (FORM == WINDOW && live != 0xffu) {
+                uint32_t sum = j ? 1u : 0u;
+#pragma unroll 1
+                for (int ks = 0; ks < 8; ++ks) {
+                  if (!((live >> ks) & 1u)) continue;
+                  tc_mma_ta(tmem + 256u + 128u * i, tmem + 128u * i + 8u * ks,
+                            v_desc + (uint64_t)(vs * (AP_TILE >> 4) + ks * (2048 >> 4)), idesc_pv, sum);
+                  sum = 1u;
+                }
+              } else if (keys >= AP_KEYS) {
 #pragma unroll
                 for (int ks = 0; ks < 8; ++ks)
                   tc_mma_ta(tmem + 256u + 128u * i, tmem + 128u * i + 8u * ks,
@@ -385,16 +485,29 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
       }
       tc_fence_after();
     };
-    for (int r = 0; r * (int)gridDim.x < sh.items; ++r) {
+    for (int r = 0; r * (int)gridDim.x < items; ++r) {
       const int w = item_of(r);
-      if (w >= sh.items) continue;
-      const Item it = item_at(sh, w, pos);
-      const int t = it.q0 + i * sh.tokens + (row >> sh.gshift);
-      const int limit = t < sh.T ? pos + t + 1 : 0;        // a row past the prompt sees nothing
-      // keys that every row of this warp sees: tiles inside them need no mask
-      const int t_first = it.q0 + i * sh.tokens + (((warp & 3) * 32) >> sh.gshift);
-      const int t_last = it.q0 + i * sh.tokens + (((warp & 3) * 32 + 31) >> sh.gshift);
-      const int free_keys = t_last < sh.T ? pos + t_first + 1 : 0;
+      if (w >= items) continue;
+      const Item it = item_of_form<FORM>(sh, w, pos, pos_ptr);
+      // token and head of the row (128 rows hold `tokens` tokens of G heads; with an odd G the last rows are nobody's)
+      const int tok = FORM == CAUSAL ? row >> sh.gshift : row / sh.G;
+      const int t = it.q0 + i * sh.tokens + tok;
+      const bool live_row = t < sh.T && (FORM == CAUSAL || tok < sh.tokens);
+      int limit, free_keys, low = 0, free_from = 0;        // the row sees [low, limit) and the sinks
+      if constexpr (FORM == CAUSAL) {
+        limit = t < sh.T ? pos + t + 1 : 0;                // a row past the prompt sees nothing
+        // keys that every row of this warp sees: tiles inside them need no mask
+        const int t_first = it.q0 + i * sh.tokens + (((warp & 3) * 32) >> sh.gshift);
+        const int t_last = it.q0 + i * sh.tokens + (((warp & 3) * 32 + 31) >> sh.gshift);
+        free_keys = t_last < sh.T ? pos + t_first + 1 : 0;
+      } else if constexpr (FORM == WINDOW) {
+        limit = min(it.pos + t + 1, sh.room);
+        low = it.pos + t + 1 - sh.window;
+        free_keys = min(it.pos + it.q0 + i * sh.tokens + (warp & 3) * 32 / sh.G + 1, sh.room);
+        free_from = it.pos + it.q0 + i * sh.tokens + ((warp & 3) * 32 + 31) / sh.G + 1 - sh.window;
+      } else {
+        limit = free_keys = pos;
+      }
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < it.n; ++j, ++step) {
         wait(bar(B_SF, i), step & 1);
@@ -412,17 +525,42 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
 #pragma unroll
           for (int k = 0; k < 16; ++k) { v[k] = lo[k]; v[k + 16] = hi[k]; }
         }
-        const int key_base = j * AP_KEYS;
+        const int key_base = key_base_of<FORM>(it, j);
         if (!plain) {
 #pragma unroll
           for (int k = 0; k < COLS; ++k) v[k] *= sh.scale_log2;
         }
-        if (key_base + AP_KEYS > free_keys) {
+        if (FORM == WINDOW) {
+          if (key_base + AP_KEYS > free_keys || (key_base < free_from && key_base + AP_KEYS > sh.sinks)) {
+            const int vis = limit - key_base - COLS * part, from = low - key_base - COLS * part,
+                      sunk = sh.sinks - key_base - COLS * part;
+#pragma unroll
+            for (int k = 0; k < COLS; ++k) v[k] = k < vis && (k >= from || k < sunk) ? v[k] : -INFINITY;
+          }
+        } else if (key_base + AP_KEYS > free_keys) {
           const int vis = limit - key_base - COLS * part;
 #pragma unroll
           for (int k = 0; k < COLS; ++k) v[k] = k < vis ? v[k] : -INFINITY;
         }
-        if (tid < 128 && key_base + AP_KEYS > it.max_limit && (it.max_limit & 15)) {
+        if (FORM == WINDOW) {
+          // V rows that no row of the item sees are cleared where their k step takes part in P V
+          if (tid < 128 && (key_base + AP_KEYS > it.max_limit || key_base < it.low)) {
+            const int key = key_base + tid;
+            const bool stale = ((live_steps<FORM>(sh, it, key_base) >> (tid >> 4)) & 1u) &&
+                               (key >= it.max_limit || (key < it.low && key >= sh.sinks));
+            if (__any_sync(0xffffffffu, stale)) {
+              wait(bar(B_VF, step & 1), (step >> 1) & 1);
+              if (stale && !broken) {
+                unsigned char* vt = smem + AP_V + (step & 1) * AP_TILE + tid * 128;
+#pragma unroll
+                for (int q = 0; q < 16; ++q)
+                  *reinterpret_cast<uint4*>(vt + (q & 8 ? AP_HALF : 0u) + ((q & 7) << 4)) = make_uint4(0, 0, 0, 0);
+              }
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+            }
+          }
+        } else if (tid < 128 && key_base + AP_KEYS > it.max_limit && (it.max_limit & 15)) {
           // V rows past the newest key hold stale bits (0 * garbage could be NaN): clear those of its
           // k step before the first product with this tile may start
           wait(bar(B_VF, step & 1), (step >> 1) & 1);
@@ -513,13 +651,36 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
       }
       wait(bar(B_OF, i), nitems & 1);
       if (broken) { ++nitems; continue; }
+      if constexpr (FORM == PARTS) {
+        const size_t prow = sh.parts.row(it.split, it.kh, (size_t)t * sh.G + (row - tok * sh.G));
+        float* to = sh.parts.o + prow * 128 + COLS * part;
+        if (live_row && part == 0) sh.parts.ml[prow] = make_float2(m * c, l);
+#pragma unroll 1
+        for (int k = 0; k < COLS / 16; ++k) {
+          float o[16];
+          tc_ld16(o_addr + 16 * k, o);
+          if (live_row) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<float4*>(to + 16 * k + 4 * q) = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+          }
+          __syncwarp();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_OE, i));
+        __syncwarp();
+        ++nitems;
+        continue;
+      }
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // NaN stays NaN
-      bf16* dst = out + (((size_t)it.b * sh.T + t) * sh.nq + it.kh * sh.G + (row & (sh.G - 1))) * 128 + COLS * part;
+      const int head = FORM == CAUSAL ? row & (sh.G - 1) : row - tok * sh.G;
+      bf16* dst = out + (((size_t)it.b * sh.T + t) * sh.nq + it.kh * sh.G + head) * 128 + COLS * part;
 #pragma unroll 1
       for (int k = 0; k < COLS / 16; ++k) {
         float o[16];
         tc_ld16(o_addr + 16 * k, o);
-        if (t < sh.T) {
+        if (live_row) {
           uint32_t u[8];
 #pragma unroll
           for (int q = 0; q < 8; ++q) u[q] = pack_bf16(o[2 * q] * inv, o[2 * q + 1] * inv);
@@ -552,41 +713,48 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
   }
 }
 
-}  // namespace
-
-extern "C" int q_attention_prefill(const void* d_q, const q_kv_layout_t* kv, const int32_t* d_pos,
-                                   void* d_out, int batch, int T, int n_q_heads, float scale,
-                                   void* stream) {
-  const char* who = "q_attention_prefill";
-  Q_CHECK_ARG(d_q && kv && d_pos && d_out, "q_attention_prefill: null pointer");
+// What q_attention_prefill, its windowed form and the partial form share. FORM WINDOW and PARTS fill their own
+// fields of `sh` before; d_out null for PARTS.
+template <int FORM>
+int prompt_launch(const char* who, AttnShape& sh, const void* d_q, const q_kv_layout_t* kv, const int32_t* d_pos,
+                  void* d_out, int batch, int T, int n_q_heads, float scale, void* stream) {
+  Q_CHECK_ARG(d_q && kv && d_pos && (d_out || FORM == PARTS), "%s: null pointer", who);
   Q_CHECK_ARG(kv->d_kpool && kv->d_vpool && kv->d_block_table && kv->pages_per_seq >= 1 &&
                   kv->n_kv_heads >= 1,
-              "q_attention_prefill: incomplete KV layout");
+              "%s: incomplete KV layout", who);
   const int nkv = kv->n_kv_heads;
   Q_CHECK_ARG(batch >= 1 && batch <= 65535 && nkv <= 65535 && T >= 1 && n_q_heads >= nkv &&
                   n_q_heads % nkv == 0,
-              "q_attention_prefill: bad batch/T/heads");
+              "%s: bad batch/T/heads", who);
   const int G = n_q_heads / nkv;
-  Q_CHECK_ARG(G <= 8 && (G & (G - 1)) == 0,
-              "q_attention_prefill: %d query heads per kv head (1, 2, 4 or 8 supported)", G);
+  if (FORM == CAUSAL) {
+    Q_CHECK_ARG(G <= 8 && (G & (G - 1)) == 0,
+                "%s: %d query heads per kv head (1, 2, 4 or 8 supported)", who, G);
+  } else {
+    Q_CHECK_ARG(G <= 32, "%s: %d query heads per kv head exceed 32", who, G);
+    Q_CHECK_ARG(kv->pages_per_seq <= (1 << 23), "%s: too many pages per sequence", who);
+    Q_CHECK_ALIGN(d_pos, 4, who); Q_CHECK_ALIGN(kv->d_block_table, 4, who);
+  }
   Q_CHECK_ALIGN(d_q, 16, who); Q_CHECK_ALIGN(d_out, 4, who);
   Q_CHECK_ALIGN(kv->d_kpool, 16, who); Q_CHECK_ALIGN(kv->d_vpool, 16, who);
   int* status = q_attn_status_addr();
   if (!status) { q_set_error("%s: could not locate the device status word", who); return Q_ERR_CUDA; }
-  AttnShape sh;
   sh.batch = batch; sh.T = T; sh.G = G; sh.nq = n_q_heads; sh.nkv = nkv; sh.pages_per_seq = kv->pages_per_seq;
+  sh.room = FORM == CAUSAL ? 0 : kv->pages_per_seq * Q_PAGE_TOKENS;
   sh.gshift = 0;
   while ((1 << sh.gshift) < G) ++sh.gshift;
-  sh.tokens = 128 >> sh.gshift;
+  sh.tokens = 128 / G;
   // Two tiles of a CTA hide each other's latencies; one tile has all 16 softmax warps, four threads to a row, and a
   // shorter chain. Up to two tiles per SM the one is faster. One tile / two, us: 1 x 592 tokens 15.5 / 18.8, 1 x 1024
   // 22.8 / 26.4, 1 x 1184 (296 tiles) 28.8 / 30.7, 3 x 250 10.2 / 12.8, 9 x 128 10.2 / 10.5, but 1 x 1200 32.4 / 31.8,
   // 3 x 400 (312) 19.4 / 17.0, 2 x 701 26.9 / 22.8. (With half of the warps idle, one tile took 17.1 at 592.)
   const int sms = q_sm_count();
-  sh.tiles = (long long)((T + sh.tokens - 1) / sh.tokens) * batch * nkv <= 2ll * sms ? 1 : 2;
-  sh.blocks = (T + sh.tiles * sh.tokens - 1) / (sh.tiles * sh.tokens);
-  const long long items = (long long)sh.blocks * batch * nkv;
-  Q_CHECK_ARG(items < (1ll << 30) && (long long)batch * T < (1ll << 31), "q_attention_prefill: too many rows");
+  const long long row_tiles = (T + sh.tokens - 1) / sh.tokens;
+  if (FORM == PARTS) sh.tiles = row_tiles == 1 ? 1 : 2;
+  else sh.tiles = row_tiles * batch * nkv <= 2ll * sms ? 1 : 2;
+  sh.blocks = (int)((row_tiles + sh.tiles - 1) / sh.tiles);
+  const long long items = (long long)sh.blocks * batch * nkv * (FORM == PARTS ? sh.parts.splits : 1);
+  Q_CHECK_ARG(items < (1ll << 30) && (long long)batch * T < (1ll << 31), "%s: too many rows", who);
   sh.items = (int)items;
   sh.wide = ((uintptr_t)d_out & 31) == 0;
   sh.scale_log2 = scale * 1.4426950408889634f;
@@ -608,10 +776,44 @@ extern "C" int q_attention_prefill(const void* d_q, const q_kv_layout_t* kv, con
     if (rc) return rc;
   }
   static size_t done[2][64] = {{0}};
-  auto kern = sh.tiles == 2 ? k_attn_prompt<2> : k_attn_prompt<1>;
+  auto kern = sh.tiles == 2 ? k_attn_prompt<2, FORM> : k_attn_prompt<1, FORM>;
   Q_CHECK_CUDA(q_ensure_smem(kern, AP_SMEM, done[sh.tiles - 1]));
   const int grid = sh.items < sms ? sh.items : sms;
   Q_CHECK_CUDA(q_launch(kern, dim3(grid), dim3(AP_THREADS), AP_SMEM, (cudaStream_t)stream, qmap, kmap, vmap,
                         kv->d_block_table, d_pos, (bf16*)d_out, sh, status));
   return Q_OK;
+}
+
+}  // namespace
+
+extern "C" int q_attention_prefill(const void* d_q, const q_kv_layout_t* kv, const int32_t* d_pos,
+                                   void* d_out, int batch, int T, int n_q_heads, float scale,
+                                   void* stream) {
+  AttnShape sh = {};
+  return prompt_launch<CAUSAL>("q_attention_prefill", sh, d_q, kv, d_pos, d_out, batch, T, n_q_heads, scale, stream);
+}
+
+extern "C" int q_attention_window_prefill(const void* d_q, const q_kv_layout_t* kv, const int32_t* d_pos,
+                                          int pos_per_seq, void* d_out, int batch, int T, int n_q_heads, int window,
+                                          int sinks, float scale, void* stream) {
+  const char* who = "q_attention_window_prefill";
+  Q_CHECK_ARG(window >= 1 && sinks >= 0, "%s: window %d / sinks %d", who, window, sinks);
+  AttnShape sh = {};
+  sh.pos_step = pos_per_seq ? 1 : 0;
+  sh.window = window < (1 << 30) ? window : 1 << 30;
+  sh.sinks = sinks < (1 << 30) ? sinks : 1 << 30;
+  return prompt_launch<WINDOW>(who, sh, d_q, kv, d_pos, d_out, batch, T, n_q_heads, scale, stream);
+}
+
+int q_attention_parts_tc(const void* d_q, const q_kv_layout_t* kv, const int32_t* d_len, float* parts_o,
+                         float* parts_ml, int splits, int tokens, int n_q_heads, float scale, void* stream) {
+  AttnShape sh = {};
+  sh.parts.o = parts_o;
+  sh.parts.ml = reinterpret_cast<float2*>(parts_ml);
+  sh.parts.keys = d_len;
+  sh.parts.splits = splits;
+  sh.parts.nkv = kv->n_kv_heads;
+  sh.parts.rows = tokens * (n_q_heads / kv->n_kv_heads);
+  sh.parts.tile = AP_KEYS;
+  return prompt_launch<PARTS>("q_attention_shared", sh, d_q, kv, d_len, nullptr, 1, tokens, n_q_heads, scale, stream);
 }

@@ -431,7 +431,7 @@ RowsPlan rows_plan(int vh, int rows, long long pages, bool join) {
   if (sms <= 0) sms = 148;
   auto least = [](long long a, long long b) { return (int)(a < b ? a : b); };
   p.clusters = 1;
-  p.groups = p.nt == 4 ? 2 : 1;
+  p.groups = 1;
   const int per_sm = p.nt == 4 ? 1 : 2;
   p.splits = least(least(MAX_SPLITS, pages), (long long)per_sm * sms / vh);
   if (p.nt == 1) {
@@ -452,9 +452,7 @@ RowsPlan rows_plan(int vh, int rows, long long pages, bool join) {
   if (each < p.stages) p.stages = (int)each;
   // a stage always belongs to the same group of warps, which tracks its parity
   if (p.groups == 3) p.stages = 3;
-  if (p.groups == 2) p.stages += p.stages & 1;
   if (p.stages < need) p.stages = need;
-  if (p.groups == 2) p.stages += p.stages & 1;
   p.share = ((rows * 128 + p.splits - 1) / p.splits + 31) / 32 * 32;
   p.smem = (size_t)p.stages * ROW_STAGE + p.nt * 8 * 256 + 16 * p.stages + 16 + (size_t)(p.splits * p.share + p.splits * rows * 2) * 4;
   return p;
@@ -474,7 +472,7 @@ int rows_launch(const RowsPlan& p, RowsArgs& a, int vh, const char* who, cudaStr
   if (!status) { q_set_error("%s: could not locate the device status word", who); return Q_ERR_CUDA; }
   a.share = p.share;
   a.stages = p.stages;
-  if (p.nt == 4) Q_CHECK_CUDA((rows_go<4, 2>(p, a, vh, status, stream)));
+  if (p.nt == 4) Q_CHECK_CUDA((rows_go<4, 1>(p, a, vh, status, stream)));
   else if (p.nt == 2) Q_CHECK_CUDA((rows_go<2, 1>(p, a, vh, status, stream)));
   else if (p.groups == 3) Q_CHECK_CUDA((rows_go<1, 3>(p, a, vh, status, stream)));
   else Q_CHECK_CUDA((rows_go<1, 1>(p, a, vh, status, stream)));
@@ -535,4 +533,85 @@ extern "C" int q_attention_window(const void* d_q, const q_kv_layout_t* kv, cons
   if (pages > all) pages = all;
   const RowsPlan p = rows_plan(batch * kv->n_kv_heads, T * a.G, pages, true);
   return rows_launch(p, a, batch * kv->n_kv_heads, who, (cudaStream_t)stream);
+}
+
+namespace {
+
+// How the prefix of a batch is split: few rows per kv head on k_attn_rows (clusters of CTAs, each leaving one
+// part), more on the prompt attention's kernel (rows there fill tiles of 128).
+struct SharedPlan { bool few; int parts, rows; RowsPlan plan; };
+
+SharedPlan shared_plan(int batch, int T, int n_q_heads, int nkv, long long prefix_pages) {
+  SharedPlan s;
+  const int G = n_q_heads / nkv;
+  s.rows = batch * T * G;
+  s.few = s.rows <= 32;
+  if (s.few) {
+    s.plan = rows_plan(nkv, s.rows, prefix_pages, false);
+    s.parts = s.plan.clusters;
+  } else {
+    int sms = q_sm_count();
+    if (sms <= 0) sms = 148;
+    const int tokens = 128 / G, tiles = (batch * T + tokens - 1) / tokens, blocks = tiles == 1 ? 1 : (tiles + 1) / 2;
+    long long n = sms / ((long long)nkv * blocks);
+    if (n > (prefix_pages + 1) / 2) n = (prefix_pages + 1) / 2;
+    s.parts = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+  }
+  return s;
+}
+
+bool shared_sizes(int batch, int T, int n_q_heads, int nkv, long long prefix_pages) {
+  return batch >= 1 && T >= 1 && nkv >= 1 && n_q_heads >= nkv && n_q_heads % nkv == 0 && (long long)T * (n_q_heads / nkv) <= 32 &&
+         (long long)batch * nkv <= 65535 && (long long)batch * T * (n_q_heads / nkv) <= (1 << 24) && prefix_pages >= 1 &&
+         prefix_pages <= (1 << 23);
+}
+
+}  // namespace
+
+extern "C" int64_t q_attention_shared_scratch_bytes(int batch, int T, int n_q_heads, int n_kv_heads, int prefix_pages) {
+  if (!shared_sizes(batch, T, n_q_heads, n_kv_heads, prefix_pages)) return 0;
+  const SharedPlan s = shared_plan(batch, T, n_q_heads, n_kv_heads, prefix_pages);
+  return (int64_t)s.parts * n_kv_heads * s.rows * (128 + 2) * 4;
+}
+
+extern "C" int q_attention_shared(const void* d_q, const q_kv_layout_t* prefix, const int32_t* d_prefix_len,
+                                  const q_kv_layout_t* kv, const int32_t* d_pos, int pos_per_seq, void* d_scratch,
+                                  void* d_out, int batch, int T, int n_q_heads, float scale, void* stream) {
+  const char* who = "q_attention_shared";
+  int rc = check_rows(who, d_q, kv, d_pos, d_out, batch, T, n_q_heads);
+  if (rc) return rc;
+  Q_CHECK_ARG(prefix && d_prefix_len && d_scratch, "%s: null pointer", who);
+  Q_CHECK_ARG(prefix->d_kpool && prefix->d_vpool && prefix->d_block_table, "%s: incomplete KV layout of the prefix", who);
+  Q_CHECK_ARG(prefix->n_kv_heads == kv->n_kv_heads, "%s: prefix and sequences have different kv heads", who);
+  const int nkv = kv->n_kv_heads;
+  Q_CHECK_ARG(shared_sizes(batch, T, n_q_heads, nkv, prefix->pages_per_seq), "%s: too many rows or prefix pages", who);
+  Q_CHECK_ALIGN(d_scratch, 16, who); Q_CHECK_ALIGN(d_prefix_len, 4, who); Q_CHECK_ALIGN(prefix->d_block_table, 4, who);
+  Q_CHECK_ALIGN(prefix->d_kpool, 16, who); Q_CHECK_ALIGN(prefix->d_vpool, 16, who);
+  const SharedPlan s = shared_plan(batch, T, n_q_heads, nkv, prefix->pages_per_seq);
+  AttnParts parts = {};
+  parts.o = (float*)d_scratch;
+  parts.ml = reinterpret_cast<float2*>(parts.o + (size_t)s.parts * nkv * s.rows * 128);
+  parts.splits = s.parts;
+  parts.nkv = nkv;
+  parts.rows = s.rows;
+  if (s.few) {
+    RowsArgs a = rows_args(d_q, prefix, d_prefix_len, 0, nullptr, batch * T, n_q_heads, scale);
+    a.flat = true;
+    a.write_parts = true;
+    a.parts = parts;
+    rc = rows_launch(s.plan, a, nkv, who, (cudaStream_t)stream);
+  } else {
+    rc = q_attention_parts_tc(d_q, prefix, d_prefix_len, parts.o, (float*)parts.ml, s.parts, batch * T, n_q_heads, scale,
+                              stream);
+    parts.keys = d_prefix_len;
+    parts.tile = 128;
+  }
+  if (rc) return rc;
+  // The sequences' own keys, under the prefix's launch: what they are made of is older than it, and the parts are
+  // read at the end, behind the wait for it.
+  RowsArgs a = rows_args(d_q, kv, d_pos, pos_per_seq, d_out, T, n_q_heads, scale);
+  a.parts = parts;
+  a.early = true;
+  const RowsPlan p = rows_plan(batch * nkv, T * a.G, kv->pages_per_seq, true);
+  return rows_launch(p, a, batch * nkv, who, (cudaStream_t)stream);
 }

@@ -431,6 +431,64 @@ class WindowAttention:
         return out
 
 
+def window_prompt_attention(query: torch.Tensor, cache: PagedKV, position: torch.Tensor, tokens_per_seq: int,
+                            scale: float, window: int, sinks: int = 0) -> torch.Tensor:
+    """prompt_attention under WindowAttention's window: a block of `tokens_per_seq` prompt tokens per sequence, whose
+    keys and values the pages already hold. position is int32 [1] or [batch]. Up to 32 query heads per kv head."""
+    T = int(tokens_per_seq)
+    if T < 1:
+        raise ValueError("at least one token per sequence")
+    _paged_query(query, cache, cache.batch * T, None)
+    if not 1 <= window < 2 ** 31 or not 0 <= sinks < 2 ** 31:
+        raise ValueError("the window must hold at least one key, and sinks cannot be negative")
+    each = _positions(position, cache.batch, query.device)
+    hq = query.shape[1]
+    with torch.cuda.device(query.device):
+        out = torch.empty((cache.batch * T, hq * HEAD_DIM), dtype=torch.bfloat16, device=query.device)
+        check(lib.q_attention_window_prefill(_ptr(query), C.byref(cache.layout), _ptr(position), each, _ptr(out),
+                                             cache.batch, T, hq, int(window), int(sinks), float(scale), _stream()))
+    return out
+
+
+class SharedPrefixAttention:
+    """GQA attention of a batch of sequences that share a prefix (several continuations of one prompt): row
+    (b, t, head) attends to all of the prefix and to its own keys [0, position + t]. The prefix is read once for the
+    whole batch, instead of once per sequence as with a copy of it, or its pages, in every sequence's cache.
+
+    `prefix` is a PagedKV of one sequence, prefix_length an int32 tensor [1] (how much of it is in use); `cache` holds
+    the keys behind the prefix, slot j of it being position prefix_length + j of the sequence. Both may lie in the same
+    pools. 1..32/G query tokens per sequence, any batch. The partial results' scratch is made per call."""
+
+    def __init__(self, batch, query_heads, kv_heads, prefix_capacity, capacity, device, tokens_per_seq=1):
+        device = torch.device(device)
+        if (device.type != "cuda" or min(batch, query_heads, kv_heads, prefix_capacity, capacity, tokens_per_seq) < 1
+                or query_heads % kv_heads or tokens_per_seq * (query_heads // kv_heads) > 32):
+            raise ValueError("unsupported shared-prefix attention metadata")
+        self.batch, self.hq, self.hk, self.T = batch, query_heads, kv_heads, tokens_per_seq
+        self.prefix_capacity, self.capacity = prefix_capacity, capacity
+
+    def run(self, query, prefix: PagedKV, prefix_length, cache: PagedKV, position, scale) -> torch.Tensor:
+        """query [batch*T, Hq, 128] -> [batch*T, Hq*128]."""
+        _paged_query(query, cache, self.batch * self.T, self.hq)
+        _paged_query(query, prefix, self.batch * self.T, self.hq)
+        if cache.batch != self.batch or cache.n_kv != self.hk or cache.capacity < self.capacity:
+            raise ValueError("cache does not match this attention instance")
+        if prefix.batch != 1 or prefix.n_kv != self.hk or prefix.capacity < self.prefix_capacity:
+            raise ValueError("the prefix must be one sequence that matches this attention instance")
+        if (tuple(prefix_length.shape) != (1,) or prefix_length.dtype != torch.int32
+                or prefix_length.device != query.device):
+            raise ValueError("prefix_length must be an int32 tensor of shape [1] on the query's device")
+        each = _positions(position, self.batch, query.device)
+        need = lib.q_attention_shared_scratch_bytes(self.batch, self.T, self.hq, self.hk, prefix.pages_per_seq)
+        with torch.cuda.device(query.device):
+            out = torch.empty((self.batch * self.T, self.hq * HEAD_DIM), dtype=torch.bfloat16, device=query.device)
+            scratch = torch.empty(max(16, need), dtype=torch.uint8, device=query.device)
+            check(lib.q_attention_shared(_ptr(query), C.byref(prefix.layout), _ptr(prefix_length),
+                                         C.byref(cache.layout), _ptr(position), each, _ptr(scratch), _ptr(out),
+                                         self.batch, self.T, self.hq, float(scale), _stream()))
+        return out
+
+
 def decode_attention(qkv, q_weight, k_weight, eps, cos, sin, position, cache: PagedKV,
                      attn: SmallQueryAttention, scale) -> torch.Tensor:
     """qkv_norm_rope_cache + SmallQueryAttention.run for one token per sequence in a single

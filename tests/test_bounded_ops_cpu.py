@@ -67,3 +67,56 @@ def test_caches_over_given_pages():
                 dict(pools=(k, v), poison=1.0), dict(pools=(k[:, :1], v[:, :1]))):
         with pytest.raises(ValueError):
             ops.PagedKV(2, 2, 150, "cpu", **bad)
+
+
+def test_window_prompt_refuses_bad_arguments():
+    from starter_b200._lib import lib
+    kv = layout()
+
+    def call(q=A, kv=kv, pos=A, out=A, batch=1, T=1, nq=8, window=5, sinks=0):
+        return lib.q_attention_window_prefill(q, C.byref(kv) if kv else None, pos, 0, out, batch, T, nq, window, sinks, 0.1, None)
+    refused(call(q=None), "null")
+    refused(call(kv=None), "null")
+    refused(call(out=None), "null")
+    refused(call(q=A + 8), "aligned")
+    refused(call(out=A + 2), "aligned")
+    refused(call(pos=A + 2), "aligned")
+    refused(call(kv=layout(pages=0)), "incomplete")
+    refused(call(T=0))
+    refused(call(nq=7))
+    refused(call(nq=66), "exceed 32")
+    refused(call(window=0), "window")
+    refused(call(sinks=-1), "sinks")
+
+
+def test_shared_prefix_refuses_bad_arguments():
+    from starter_b200._lib import lib
+    kv = layout()
+
+    def call(q=A, prefix=kv, length=A, kv=kv, pos=A, scratch=A, out=A, batch=2, T=1, nq=8):
+        return lib.q_attention_shared(q, C.byref(prefix) if prefix else None, length, C.byref(kv) if kv else None, pos, 0,
+                                      scratch, out, batch, T, nq, 0.1, None)
+    for name in ("q", "prefix", "length", "kv", "pos", "scratch", "out"):
+        refused(call(**{name: None}), "null")
+    refused(call(q=A + 8), "aligned")
+    refused(call(scratch=A + 8), "aligned")
+    refused(call(length=A + 1), "aligned")
+    refused(call(prefix=layout(k=A + 8)), "aligned")
+    refused(call(prefix=layout(nkv=4)), "different kv heads")
+    refused(call(prefix=layout(v=None)), "incomplete")
+    refused(call(prefix=layout(pages=0)), "too many")
+    refused(call(nq=2, T=33), "32 query rows")
+    refused(call(batch=0))
+    assert lib.q_attention_shared_scratch_bytes(2, 1, 8, 2, 10) > 0
+    for bad in ((0, 1, 8, 2, 10), (2, 0, 8, 2, 10), (2, 1, 7, 2, 10), (2, 1, 8, 0, 10), (2, 9, 8, 2, 10), (2, 1, 8, 2, 0)):
+        assert lib.q_attention_shared_scratch_bytes(*bad) == 0
+
+
+def test_shared_prefix_class_refuses_before_a_launch():
+    from starter_b200 import ops
+    with pytest.raises(ValueError):
+        ops.SharedPrefixAttention(1, 32, 8, 0, 100, "cuda")
+    with pytest.raises(ValueError):
+        ops.SharedPrefixAttention(1, 32, 8, 100, 100, "cpu")
+    with pytest.raises(ValueError):
+        ops.SharedPrefixAttention(1, 32, 8, 100, 100, "cuda", 9)
