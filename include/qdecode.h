@@ -413,6 +413,34 @@ int q_logits_argmax(const float* d_branch, const q_gemm_plan_t* plan,
                     void* d_block_scratch, int rows, int vocab, int vocab_offset,
                     void* stream);
 
+/* ---- a token by chance ------------------------------------------------------
+ * (No reference counterpart.) From bf16 (fp32 = 0) or fp32 logits [rows][vocab], rows row_stride values apart (0: every
+ * row draws from the same logits): of every row the token that the random number d_uniform[row] in [0, 1) stands for, and the logarithm of its
+ * probability in the set it was drawn from. With w_i = exp((x_i - max x) / temperature):
+ *   top_k:  the top_k largest logits, of equal ones those of the lowest index (0, negative, vocab and more: all);
+ *   min_p:  of those the ones with w_i >= min_p, that is, of at least min_p times the largest probability (0: all);
+ *   top_p:  of those, in descending order (equal ones by index), the shortest run with a sum of w of at least
+ *           top_p times all of theirs, never less than one (1 and more: all);
+ *   token:  the first of these, by index, at which their running sum of w exceeds d_uniform[row] times
+ *           their whole sum (numbers below 0 and NaN count as 0, 1 and more take the last).
+ * temperature 0: the largest logit, of equal ones the lowest index. Logits that are -inf or NaN are never drawn; a row
+ * that has no others gives token -1 and -inf. If +inf occurs, only it is drawn. Every setting is one number or, where
+ * its pointer is set, one per row in device memory (there a NaN or negative temperature means 0, a NaN
+ * top_p or min_p that it is off). Weights and sums are exact to 2^-44 of the largest weight, and the
+ * result does not depend on the order of execution. vocab up to 2^19. One launch, no scratch. */
+typedef struct q_sampling_t {
+  float temperature;
+  int32_t top_k;
+  float top_p, min_p;
+  const float* d_temperature;   /* [rows] each, or NULL */
+  const int32_t* d_top_k;
+  const float* d_top_p;
+  const float* d_min_p;
+} q_sampling_t;
+int q_sample_tokens(const void* d_logits, int fp32, int64_t row_stride, const float* d_uniform,
+                    const q_sampling_t* sampling, int64_t* d_tokens, float* d_logprobs, int rows, int vocab,
+                    void* stream);
+
 /* Final pick over tensor-parallel shards: val/idx are [shards][rows]; lowest
  * global index wins ties. Writes tokens and bumps *d_pos like above. */
 int q_argmax_merge(const float* d_val, const int32_t* d_idx, int shards, int rows,

@@ -78,6 +78,12 @@ class Prompt(C.Structure):
                                              "act", "partials", "split")])
 
 
+class Sampling(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float),
+                ("d_temperature", C.c_void_p), ("d_top_k", C.c_void_p), ("d_top_p", C.c_void_p),
+                ("d_min_p", C.c_void_p)]
+
+
 _P = C.c_void_p
 _I = C.c_int
 _F = C.c_float
@@ -155,6 +161,7 @@ SIGNATURES = {
     "q_attention_decode": (_I, [_P, _PLAN, _P, _P, _P, _P, _P, _KV, _P, _P, _P, _P, _I, _I, _I, _F, _F, _P]),
     "q_argmax_scratch_bytes": (C.c_int64, [_I, _I]),
     "q_logits_argmax": (_I, [_P, _PLAN, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P]),
+    "q_sample_tokens": (_I, [_P, _I, C.c_int64, _P, C.POINTER(Sampling), _P, _P, _I, _I, _P]),
     "q_argmax_merge": (_I, [_P, _P, _I, _I, _P, _P, _I, _P]),
     "q_create": (_I, [C.POINTER(Config), C.POINTER(_P)]),
     "q_bind_layer": (_I, [_P, _I, C.POINTER(LayerWeights)]),

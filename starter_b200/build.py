@@ -14,7 +14,7 @@ ROOT = Path(__file__).resolve().parent
 CSRC = ROOT / "csrc"
 LIB = Path(os.environ.get("QDECODE_LIB", ROOT / "libqdecode.so"))
 SOURCES = ["capi.cu", "gemm_streamk.cu", "gemm_tc.cu", "gemm_rows.cu", "gemm_prompt.cu", "fused_ops.cu", "attention.cu",
-           "attn_prompt.cu", "attn_rows.cu"]
+           "attn_prompt.cu", "attn_rows.cu", "sampling.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",

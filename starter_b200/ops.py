@@ -529,6 +529,48 @@ def lm_head_argmax(normed: torch.Tensor, weight, return_logits: bool = True):
     return logits, tokens
 
 
+def _setting(value, rows: int, device, dtype, what: str):
+    """(number, pointer): a number for all rows, or a tensor with one per row."""
+    if not isinstance(value, torch.Tensor):
+        return value, 0
+    if tuple(value.shape) != (rows,) or value.dtype != dtype or value.device != device or not value.is_contiguous():
+        raise ValueError(f"{what} must be a number or a contiguous {dtype} tensor [rows] on the logits' device")
+    return 0, value.data_ptr()
+
+
+def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Tokens drawn from the logits by the given random numbers, beside lm_head_argmax's greedy ones: temperature,
+    then the top_k largest, then those of at least min_p times the largest probability, then the most likely ones
+    that make up top_p of what is left (q_sample_tokens says it exactly).
+
+    logits: BF16 or FP32 [rows, vocab], rows any stride apart (expanded ones too: several
+    draws from the same logits); uniform: FP32 [rows] in [0, 1). Every setting is a
+    number, or a tensor with one per row (FP32; top_k int32). temperature 0 is greedy. Returns (tokens int64 [rows],
+    logprobs FP32 [rows]): -1 and -inf for a row without a finite logit."""
+    if (logits.ndim != 2 or not logits.is_cuda or logits.dtype not in (torch.bfloat16, torch.float32)
+            or logits.shape[0] < 1 or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1)):
+        raise ValueError("logits must be a BF16 or FP32 CUDA [rows, vocab] tensor with adjacent columns")
+    rows, vocab = logits.shape
+    dev = logits.device
+    if (tuple(uniform.shape) != (rows,) or uniform.dtype != torch.float32 or uniform.device != dev
+            or not uniform.is_contiguous()):
+        raise ValueError("uniform must be a contiguous FP32 tensor [rows] on the logits' device")
+    t, dt = _setting(temperature, rows, dev, torch.float32, "temperature")
+    k, dk = _setting(top_k, rows, dev, torch.int32, "top_k")
+    p, dp = _setting(top_p, rows, dev, torch.float32, "top_p")
+    m, dm = _setting(min_p, rows, dev, torch.float32, "min_p")
+    if int(k) != k or not 0 <= k < 2 ** 31:
+        raise ValueError("top_k must be a whole number from 0 on")
+    settings = _lib.Sampling(t, int(k), p, m, dt, dk, dp, dm)
+    with torch.cuda.device(dev):
+        tokens = torch.empty(rows, dtype=torch.int64, device=dev)
+        logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
+        check(lib.q_sample_tokens(_ptr(logits), int(logits.dtype == torch.float32), logits.stride(0),
+                                  _ptr(uniform), C.byref(settings), _ptr(tokens), _ptr(logprobs), rows, vocab,
+                                  _stream()))
+    return tokens, logprobs
+
+
 def device_status() -> list[int]:
     """The four status words of the current device (synchronises): non-zero = a bounded wait
     inside a kernel ran out (attention, stream-K GEMM, tcgen05 GEMM, peer exchange)."""

@@ -120,3 +120,46 @@ def test_shared_prefix_class_refuses_before_a_launch():
         ops.SharedPrefixAttention(1, 32, 8, 100, 100, "cpu")
     with pytest.raises(ValueError):
         ops.SharedPrefixAttention(1, 32, 8, 100, 100, "cuda", 9)
+
+
+def test_sampling_refuses_bad_arguments():
+    from starter_b200._lib import Sampling, lib
+
+    def call(x=A, u=A, s=Sampling(1.0, 0, 1.0, 0.0), tokens=A, logprobs=A, rows=2, vocab=10, stride=10, fp32=1):
+        return lib.q_sample_tokens(x, fp32, stride, u, C.byref(s) if s else None, tokens, logprobs, rows, vocab, None)
+    for name in ("x", "u", "s", "tokens", "logprobs"):
+        refused(call(**{name: None}), "null")
+    refused(call(rows=0))
+    refused(call(vocab=0))
+    refused(call(vocab=2 ** 19 + 1))
+    refused(call(stride=-1), "stride")
+    refused(call(s=Sampling(-0.5, 0, 1.0, 0.0)), "temperature")
+    refused(call(s=Sampling(float("nan"), 0, 1.0, 0.0)), "temperature")
+    refused(call(s=Sampling(1.0, 0, float("nan"), 0.0)), "NaN")
+    refused(call(s=Sampling(1.0, 0, 1.0, float("nan"))), "NaN")
+    refused(call(x=A + 2), "aligned")
+    refused(call(x=A + 1, fp32=0), "aligned")
+    refused(call(tokens=A + 4), "aligned")
+    refused(call(s=Sampling(1.0, 0, 1.0, 0.0, None, A + 2)), "aligned")
+
+
+def test_sampling_operator_refuses_before_a_launch():
+    from starter_b200 import ops
+    with pytest.raises(ValueError):
+        ops.sample_tokens(torch.zeros((2, 5)), torch.zeros(2))
+
+
+def test_sampling_reference():
+    """Known answers of the definition that the GPU tests compare with."""
+    from tests.sampling_reference import sample
+    x = torch.tensor([1.0, 3.0, 2.0, 3.0])
+    assert sample(x, 0.9, temperature=0.0)[0] == 1
+    assert sample(x, 0.9, top_k=1)[0] == 1 and sample(x, 0.6, top_k=2)[0] == 3
+    p = torch.softmax(x.double(), 0)
+    for u in (0.0, 0.03, 0.5, 0.7, 0.999):
+        assert sample(x, u)[0] == int((p.cumsum(0) <= u).sum())
+    # weights 0.135, 1, 0.368, 1 of 2.503: the first of the set has 0.3995
+    assert sample(x, 0.99, top_p=0.5)[0] == 3 and sample(x, 0.99, top_p=0.39)[0] == 1
+    assert sample(x, 0.99, min_p=0.5)[0] == 3 and sample(x, 0.99, min_p=0.3)[0] == 3
+    assert sample(x, 0.45, min_p=0.3)[0] == 2                  # of ids 1, 2, 3 with weights 1, 0.37, 1
+    assert sample(torch.full((3,), -torch.inf), 0.5)[0] == -1
