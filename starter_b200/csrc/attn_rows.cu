@@ -14,9 +14,11 @@
 // keys -> join is a chain of memory round trips); hence one launch, and of a page only the rows somebody sees
 // are copied: a window with 4 sinks brings 4 rows of its first page.
 //
-// Keys are the M dimension of the MMAs, query rows (NT tiles of 8) the N dimension: S^T = K Q^T, O^T = V^T P^T,
-// as in the decode attention, so that few rows leave no accumulator empty. DG groups of four warps take a tile of
-// 64 keys each, a warp 16 keys. Cast boundaries as there: fp32 scores and statistics, P rounded to bf16 for
+// Keys are the M dimension of the MMAs, a tile of 8 query rows the N dimension: S^T = K Q^T, O^T = V^T P^T,
+// as in the decode attention, so that few rows leave no accumulator empty. Four warps share a tile of 64 keys, 16
+// keys each; RG such groups take a row tile each, DG of them a key tile each. (With the row tiles in one warp's
+// registers, four at most, a tile of 64 keys and 32 rows took 2.9 us: one warp a scheduler hides none of the MMAs'
+// latency. As here 0.9.) Cast boundaries as there: fp32 scores and statistics, P rounded to bf16 for
 // P V (the tensor cores' operand type), fp32 sums, one rounding of the result.
 //
 // Rows of a page that no query row sees may hold anything: their scores are replaced, their values cleared.
@@ -94,17 +96,17 @@ __device__ __forceinline__ uint32_t remote_addr(uint32_t local, int rank) {
   return r;
 }
 
-template <int NT, int DG>
-__global__ void __launch_bounds__((4 * DG + 1) * 32, (NT <= 2 && DG == 1) ? 2 : 1)
-k_attn_rows(const RowsArgs a, int* status) {
-  constexpr int DC = 4 * DG;                       // consumer warps
+template <int RG, int DG, int BLOCKS>
+__global__ void __launch_bounds__((4 * RG * DG + 1) * 32, BLOCKS)
+k_attn_rows(RowsArgs a, int* status) {
+  constexpr int DC = 4 * RG * DG;                  // consumer warps
   constexpr int DT = (DC + 1) * 32;
-  constexpr int SETS = NT == 1 ? 4 : NT == 2 ? 2 : 1;      // accumulators of a row tile's Q K^T
+  constexpr int SETS = 4;                          // accumulators of Q K^T: an MMA's result is ~280 cycles away
   extern __shared__ __align__(1024) unsigned char smem[];
   const int NS = a.stages;
   unsigned char* stages = smem;
-  unsigned char* qtile = smem + NS * ROW_STAGE;                            // NT * 8 rows of 256 B
-  uint64_t* bars = reinterpret_cast<uint64_t*>(qtile + NT * 8 * 256);      // full[NS], empty[NS]
+  unsigned char* qtile = smem + NS * ROW_STAGE;                            // RG * 8 rows of 256 B
+  uint64_t* bars = reinterpret_cast<uint64_t*>(qtile + RG * 8 * 256);      // full[NS], empty[NS]
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * NS);
   float* recv = reinterpret_cast<float*>(bars + 2 * NS + 2);               // [splits][share] sums, then [splits][R][2]
 
@@ -115,7 +117,7 @@ k_attn_rows(const RowsArgs a, int* status) {
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(smem_u32(&bars[i]), 1);
-      mbar_init(smem_u32(&bars[NS + i]), 4);
+      mbar_init(smem_u32(&bars[NS + i]), 4 * RG);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -173,7 +175,7 @@ k_attn_rows(const RowsArgs a, int* status) {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   } else {
     // ---------------- consumers ----------------
-    for (int c = tid; c < NT * 8 * 16; c += DC * 32) {
+    for (int c = tid; c < RG * 8 * 16; c += DC * 32) {
       const int r = c >> 4, ch = c & 15;
       uint4 v = make_uint4(0, 0, 0, 0);
       if (r < R) {
@@ -185,41 +187,29 @@ k_attn_rows(const RowsArgs a, int* status) {
     asm volatile("bar.sync 1, %0;" ::"n"(DC * 32) : "memory");
 
     const int g = lane >> 2, t4 = lane & 3;
-    float m_run[NT][2], l_run[NT][2];              // rows 8 n + 2 t4, + 1 (l: of this lane's keys)
-    float oacc[NT][8][4];                          // dims 16 d + g, 16 d + g + 8
-    int lim_r[NT][2], low_r[NT][2];                // what the row sees: [low, lim) and the sinks
+    const int wk = warp & 3;                       // key quarter of the warp
+    const int rg = (warp >> 2) % RG, tg = (warp >> 2) / RG;     // its row tile, and its tiles: tg, tg + DG, ..
+    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};   // rows 8 rg + 2 t4, + 1 (l: of this lane's keys)
+    float oacc[8][4];                              // dims 16 d + g, 16 d + g + 8
+    int lim_r[2], low_r[2];                        // what the row sees: [low, lim) and the sinks
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        m_run[n][h] = -INFINITY;
-        l_run[n][h] = 0.f;
-        const int r = 8 * n + 2 * t4 + h, t = r / a.G;
-        lim_r[n][h] = r >= R ? 0 : a.flat ? seen.lim : min(seen.pos + t + 1, seen.lim);
-        low_r[n][h] = a.flat ? 0 : seen.pos + t + 1 - a.window;
-      }
-#pragma unroll
-      for (int d = 0; d < 8; ++d) oacc[n][d][0] = oacc[n][d][1] = oacc[n][d][2] = oacc[n][d][3] = 0.f;
+    for (int h = 0; h < 2; ++h) {
+      const int r = 8 * rg + 2 * t4 + h, t = r / a.G;
+      lim_r[h] = r >= R ? 0 : a.flat ? seen.lim : min(seen.pos + t + 1, seen.lim);
+      low_r[h] = a.flat ? 0 : seen.pos + t + 1 - a.window;
     }
-    const uint32_t q_base = smem_u32(qtile);
-    uint32_t qf[NT <= 2 ? NT : 1][8][2];           // Q^T fragments; four row tiles read them from shared memory each time
-    if constexpr (NT <= 2) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+    for (int d = 0; d < 8; ++d) oacc[d][0] = oacc[d][1] = oacc[d][2] = oacc[d][3] = 0.f;
+    uint32_t qf[8][2];                             // Q^T fragments of the eight k steps
 #pragma unroll
-        for (int kp = 0; kp < 4; ++kp) {
-          const int row = 8 * n + (lane & 7), ch = 4 * kp + (lane >> 3);
-          ldsm_x4(q_base + row * 256 + ((ch ^ (row & 7)) << 4), qf[n][2 * kp][0], qf[n][2 * kp][1],
-                  qf[n][2 * kp + 1][0], qf[n][2 * kp + 1][1]);
-        }
+    for (int kp = 0; kp < 4; ++kp) {
+      const int row = 8 * rg + (lane & 7), ch = 4 * kp + (lane >> 3);
+      ldsm_x4(smem_u32(qtile) + row * 256 + ((ch ^ (row & 7)) << 4), qf[2 * kp][0], qf[2 * kp][1], qf[2 * kp + 1][0], qf[2 * kp + 1][1]);
     }
-    const int grp = warp >> 2, wk = warp & 3;      // tile lane of the warp's group, key quarter of the warp
-    bool ok = true;
-    for (int it = grp; it < ntiles; it += DG) {
+    for (int it = tg; it < ntiles; it += DG) {
       const int s = it % NS;
       const int landed = mbar_wait(smem_u32(&bars[s]), (it / NS) & 1, abort_flag) ? 1 : 0;
-      ok = __all_sync(0xffffffffu, landed);
-      if (!ok) {
+      if (!__all_sync(0xffffffffu, landed)) {
         if (lane == 0) { atomicExch(status, 2); *abort_flag = 1; }
         break;
       }
@@ -228,7 +218,8 @@ k_attn_rows(const RowsArgs a, int* status) {
       const int key0 = page_of(seen, first + it) * Q_PAGE_TOKENS + wk * 16;
       if (key0 < seen.lim && (key0 + 16 > seen.low || key0 < a.sinks)) {
         if (key0 + 16 > seen.lim || (key0 < seen.low && key0 + 16 > a.sinks)) {
-          // values that no row sees are cleared: 0 * garbage could be NaN in P V
+          // values that no row sees are cleared: 0 * garbage could be NaN in P V (the warps of the other row tiles
+          // write the same zeros)
           for (int i = lane; i < 16 * 16; i += 32) {
             const int key = key0 + (i >> 4);
             if (key >= seen.lim || (key < seen.low && key >= a.sinks))
@@ -238,121 +229,96 @@ k_attn_rows(const RowsArgs a, int* status) {
           __syncwarp();
         }
         const uint32_t k_base = smem_u32(kt), v_base = smem_u32(vt);
-        float sset[NT][SETS][4];
+        float sset[SETS][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int q = 0; q < SETS; ++q) sset[n][q][0] = sset[n][q][1] = sset[n][q][2] = sset[n][q][3] = 0.f;
+        for (int q = 0; q < SETS; ++q) sset[q][0] = sset[q][1] = sset[q][2] = sset[q][3] = 0.f;
         const int arow = wk * 16 + (lane & 7) + 8 * ((lane >> 3) & 1);
 #pragma unroll
-        for (int kp = 0; kp < 4; ++kp) {
-          uint32_t ka[2][4];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int ch = 2 * (2 * kp + e) + (lane >> 4);
-            ldsm_x4(k_base + arow * 256 + ((ch ^ (arow & 7)) << 4), ka[e][0], ka[e][1], ka[e][2], ka[e][3]);
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            uint32_t q0, q1, q2, q3;
-            if constexpr (NT <= 2) {
-              q0 = qf[n][2 * kp][0]; q1 = qf[n][2 * kp][1]; q2 = qf[n][2 * kp + 1][0]; q3 = qf[n][2 * kp + 1][1];
-            } else {
-              const int row = 8 * n + (lane & 7), ch = 4 * kp + (lane >> 3);
-              ldsm_x4(q_base + row * 256 + ((ch ^ (row & 7)) << 4), q0, q1, q2, q3);
-            }
-            mma16816(sset[n][(2 * kp) % SETS], ka[0][0], ka[0][1], ka[0][2], ka[0][3], q0, q1);
-            mma16816(sset[n][(2 * kp + 1) % SETS], ka[1][0], ka[1][1], ka[1][2], ka[1][3], q2, q3);
-          }
+        for (int ks = 0; ks < 8; ++ks) {
+          uint32_t a0, a1, a2, a3;
+          const int ch = 2 * ks + (lane >> 4);
+          ldsm_x4(k_base + arow * 256 + ((ch ^ (arow & 7)) << 4), a0, a1, a2, a3);
+          mma16816(sset[ks % SETS], a0, a1, a2, a3, qf[ks][0], qf[ks][1]);
         }
         // every row sees all 16 keys: nothing to mask
         const bool open = key0 + 16 <= (a.flat ? seen.lim : seen.pos + 1) &&
                           (a.flat || key0 > seen.pos + a.T - 1 - a.window || key0 + 16 <= a.sinks);
-        uint32_t pb[NT][2];
+        float sc[4];                             // (key g, row 2 t4), (g, 2 t4 + 1), (g + 8, 2 t4), (g + 8, 2 t4 + 1)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float sc[4];                           // (key g, row 2 t4), (g, 2 t4 + 1), (g + 8, 2 t4), (g + 8, 2 t4 + 1)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float v = sset[n][0][e];
-            if (SETS == 2) v += sset[n][1][e];
-            if (SETS == 4) v = (v + sset[n][1][e]) + (sset[n][2][e] + sset[n][3][e]);
-            v *= a.scale_log2;
-            if (!open) {
-              const int key = key0 + g + 8 * (e >> 1);
-              v = key < lim_r[n][e & 1] && (key >= low_r[n][e & 1] || key < a.sinks) ? v : -INFINITY;
-            }
-            sc[e] = v;
+        for (int e = 0; e < 4; ++e) {
+          float v = ((sset[0][e] + sset[1][e]) + (sset[2][e] + sset[3][e])) * a.scale_log2;
+          if (!open) {
+            const int key = key0 + g + 8 * (e >> 1);
+            v = key < lim_r[e & 1] && (key >= low_r[e & 1] || key < a.sinks) ? v : -INFINITY;
           }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float mx = fmaxf(sc[h], sc[2 + h]);
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            const float m_new = fmaxf(m_run[n][h], mx);
-            const float m_safe = m_new == -INFINITY ? 0.f : m_new;
-            const float resc = exp2f(m_run[n][h] - m_safe);          // exp2(-inf) = 0 on the first keys
-            sc[h] = exp2f(sc[h] - m_safe);
-            sc[2 + h] = exp2f(sc[2 + h] - m_safe);
-            l_run[n][h] = l_run[n][h] * resc + (sc[h] + sc[2 + h]);
-            m_run[n][h] = m_new;
-#pragma unroll
-            for (int d = 0; d < 8; ++d) { oacc[n][d][h] *= resc; oacc[n][d][2 + h] *= resc; }
-          }
-          pb[n][0] = transpose8x8(pack_bf16(sc[0], sc[1]));
-          pb[n][1] = transpose8x8(pack_bf16(sc[2], sc[3]));
+          sc[e] = v;
         }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float mx = fmaxf(sc[h], sc[2 + h]);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float m_new = fmaxf(m_run[h], mx);
+          const float m_safe = m_new == -INFINITY ? 0.f : m_new;
+          const float resc = exp2f(m_run[h] - m_safe);               // exp2(-inf) = 0 on the first keys
+          sc[h] = exp2f(sc[h] - m_safe);
+          sc[2 + h] = exp2f(sc[2 + h] - m_safe);
+          l_run[h] = l_run[h] * resc + (sc[h] + sc[2 + h]);
+          m_run[h] = m_new;
+#pragma unroll
+          for (int d = 0; d < 8; ++d) { oacc[d][h] *= resc; oacc[d][2 + h] *= resc; }
+        }
+        const uint32_t pb0 = transpose8x8(pack_bf16(sc[0], sc[1])), pb1 = transpose8x8(pack_bf16(sc[2], sc[3]));
         const int mi = lane >> 3, vrow = wk * 16 + 8 * (mi >> 1) + (lane & 7);
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
           uint32_t v0, v1, v2, v3;
           const int ch = 2 * d + (mi & 1);
           ldsm_x4_t(v_base + vrow * 256 + ((ch ^ (vrow & 7)) << 4), v0, v1, v2, v3);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816(oacc[n][d], v0, v1, v2, v3, pb[n][0], pb[n][1]);
+          mma16816(oacc[d], v0, v1, v2, v3, pb0, pb1);
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bars[NS + s]));
     }
-    // join the consumer warps' states through shared memory (the R real rows), over the ring: every copy has
+    // join the warps' states of a row through shared memory (the R real rows), over the ring: every copy has
     // landed, since every tile was waited for
     asm volatile("bar.sync 1, %0;" ::"n"(DC * 32) : "memory");
-    float* mo = reinterpret_cast<float*>(stages);            // [DC][R][ROW_LD]
-    float* mml = mo + DC * R * ROW_LD;                       // [DC][R][2]
+    constexpr int STATES = 4 * DG;                           // of a row
+    float* mo = reinterpret_cast<float*>(stages);            // [STATES][R][ROW_LD]
+    float* mml = mo + STATES * R * ROW_LD;                   // [STATES][R][2]
     if (*abort_flag == 0) {
+      const int state = tg * 4 + wk;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int h = 0; h < 2; ++h) {
+        float l = l_run[h];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        const int r = 8 * rg + 2 * t4 + h;
+        if (r < R) {
+          float* dst = mo + (state * R + r) * ROW_LD + g;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float l = l_run[n][h];
-          l += __shfl_xor_sync(0xffffffffu, l, 4);
-          l += __shfl_xor_sync(0xffffffffu, l, 8);
-          l += __shfl_xor_sync(0xffffffffu, l, 16);
-          const int r = 8 * n + 2 * t4 + h;
-          if (r < R) {
-            float* dst = mo + (warp * R + r) * ROW_LD + g;
-#pragma unroll
-            for (int d = 0; d < 8; ++d) { dst[16 * d] = oacc[n][d][h]; dst[16 * d + 8] = oacc[n][d][2 + h]; }
-            if (g == 0) {
-              mml[(warp * R + r) * 2] = m_run[n][h];
-              mml[(warp * R + r) * 2 + 1] = l;
-            }
+          for (int d = 0; d < 8; ++d) { dst[16 * d] = oacc[d][h]; dst[16 * d + 8] = oacc[d][2 + h]; }
+          if (g == 0) {
+            mml[(state * R + r) * 2] = m_run[h];
+            mml[(state * R + r) * 2 + 1] = l;
           }
         }
+      }
     }
     asm volatile("bar.sync 1, %0;" ::"n"(DC * 32) : "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     const int d = tid & 127;
-    for (int r = tid >> 7; r < R && *abort_flag == 0; r += DG) {
-      float mw[DC], Mx = -INFINITY;
+    for (int r = tid >> 7; r < R && *abort_flag == 0; r += RG * DG) {
+      float mw[STATES], Mx = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < DC; ++w) { mw[w] = mml[(w * R + r) * 2]; Mx = fmaxf(Mx, mw[w]); }
+      for (int w = 0; w < STATES; ++w) { mw[w] = mml[(w * R + r) * 2]; Mx = fmaxf(Mx, mw[w]); }
       const float Ms = Mx == -INFINITY ? 0.f : Mx;
       float Lsum = 0.f, O = 0.f;
 #pragma unroll
-      for (int w = 0; w < DC; ++w) {
+      for (int w = 0; w < STATES; ++w) {
         const float wt = exp2f(mw[w] - Ms);
         Lsum += wt * mml[(w * R + r) * 2 + 1];
         O += wt * mo[(w * R + r) * ROW_LD + d];
@@ -419,52 +385,87 @@ k_attn_rows(const RowsArgs a, int* status) {
   }
 }
 
-// How a launch splits: CTAs of a cluster, clusters of a (sequence, kv head), warp groups, ring stages.
-struct RowsPlan { int nt, groups, splits, clusters, stages, share; size_t smem; };
+// How a launch splits: row tiles, tile groups, CTAs of a cluster, clusters of a (sequence, kv head), ring stages.
+struct RowsPlan { int rg, dg, splits, clusters, stages, share; size_t smem; };
 
-// vh: (sequence, kv head) pairs; pages: most pages a pair's rows can see. join: the splits merge in one
-// cluster; otherwise the pages go to as many clusters as fill the SMs.
-RowsPlan rows_plan(int vh, int rows, long long pages, bool join) {
-  RowsPlan p;
-  p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
-  int sms = q_sm_count();
-  if (sms <= 0) sms = 148;
-  auto least = [](long long a, long long b) { return (int)(a < b ? a : b); };
-  p.clusters = 1;
-  p.groups = 1;
-  const int per_sm = p.nt == 4 ? 1 : 2;
-  p.splits = least(least(MAX_SPLITS, pages), (long long)per_sm * sms / vh);
-  if (p.nt == 1) {
-    // every CTA an SM of its own, three groups of warps: the tiles of a split side by side
-    const int wide = least(least(MAX_SPLITS, (pages - 1) / 2), sms / vh);
-    if (wide >= 2) { p.groups = 3; p.splits = wide; }
-  }
-  if (p.splits < 1) p.splits = 1;
-  if (!join) {
-    p.clusters = least(pages / p.splits, (long long)(p.groups == 1 ? per_sm : 1) * sms / ((long long)vh * p.splits));
-    if (p.clusters < 1) p.clusters = 1;
-    if (p.clusters > 64) p.clusters = 64;
-  }
-  const long long each = (pages + (long long)p.splits * p.clusters - 1) / ((long long)p.splits * p.clusters);
-  const int dc = 4 * p.groups;
-  p.stages = p.nt == 4 ? 6 : 3;
-  const int need = (dc * rows * (ROW_LD + 2) * 4 + ROW_STAGE - 1) / ROW_STAGE;       // the warps' states lie over the ring
-  if (each < p.stages) p.stages = (int)each;
-  // a stage always belongs to the same group of warps, which tracks its parity
-  if (p.groups == 3) p.stages = 3;
-  if (p.stages < need) p.stages = need;
-  p.share = ((rows * 128 + p.splits - 1) / p.splits + 31) / 32 * 32;
-  p.smem = (size_t)p.stages * ROW_STAGE + p.nt * 8 * 256 + 16 * p.stages + 16 + (size_t)(p.splits * p.share + p.splits * rows * 2) * 4;
-  return p;
+typedef void (*rows_kernel)(RowsArgs, int*);
+rows_kernel rows_form(const RowsPlan& p) {
+  if (p.rg == 4) return k_attn_rows<4, 1, 1>;
+  if (p.rg == 2) return k_attn_rows<2, 1, 2>;
+  return p.dg == 3 ? k_attn_rows<1, 3, 1> : k_attn_rows<1, 1, 3>;
 }
 
-template <int NT, int DG>
-cudaError_t rows_go(const RowsPlan& p, const RowsArgs& a, int vh, int* status, cudaStream_t stream) {
-  static size_t done[64] = {0};
-  cudaError_t e = q_ensure_smem(k_attn_rows<NT, DG>, p.smem, done);
-  if (e != cudaSuccess) return e;
-  return q_launch_cluster(k_attn_rows<NT, DG>, dim3(p.splits * p.clusters, vh), dim3((4 * DG + 1) * 32), p.smem, stream,
-                          (unsigned)p.splits, a, status);
+size_t rows_smem(const RowsPlan& p, int rows) {
+  return (size_t)p.stages * ROW_STAGE + p.rg * 8 * 256 + 16 * p.stages + 16 + (size_t)(p.splits * p.share + p.splits * rows * 2) * 4;
+}
+
+// Fills in the ring and the sizes for `each` pages a split.
+void rows_sizes(RowsPlan& p, int rows, long long each) {
+  p.stages = p.rg == 4 ? 6 : 3;
+  const int need = (4 * p.dg * rows * (ROW_LD + 2) * 4 + ROW_STAGE - 1) / ROW_STAGE;       // the warps' states lie over the ring
+  if (each < p.stages) p.stages = each < 1 ? 1 : (int)each;
+  if (p.dg == 3) p.stages = 3;                    // a stage always belongs to the same group, which tracks its parity
+  if (p.stages < need) p.stages = need;
+  p.share = ((rows * 128 + p.splits - 1) / p.splits + 31) / 32 * 32;
+  p.smem = rows_smem(p, rows);
+}
+
+// Clusters of a form that the current device holds at once (a cluster stays inside one GPC, so this is less than
+// the SMs would allow), asked once per device.
+int rows_resident(const RowsPlan& p) {
+  static int cached[64][4][MAX_SPLITS + 1];
+  const int form = p.rg == 4 ? 3 : p.rg == 2 ? 2 : p.dg == 3 ? 1 : 0;
+  const int dev = q_device_index(), per_sm = form == 0 || form == 2 ? 2 : 1;
+  if (dev < 0) return per_sm * 148 / p.splits;
+  int& n = cached[dev][form][p.splits];
+  if (n == 0) {
+    RowsPlan full = p;
+    rows_sizes(full, 8 * p.rg, 1 << 20);
+    const rows_kernel k = rows_form(full);
+    int got = 0;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)full.smem);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.splits);
+    cfg.blockDim = dim3((4 * p.rg * p.dg + 1) * 32);
+    cfg.dynamicSmemBytes = full.smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = p.splits; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&got, k, &cfg);
+    if (e != cudaSuccess) { cudaGetLastError(); got = per_sm * 148 / p.splits; }
+    n = got > 0 ? got : -1;
+  }
+  return n;
+}
+
+// vh: (sequence, kv head) pairs; pages: most pages a pair's rows can see. join: the splits merge in one
+// cluster; otherwise the pages go to as many clusters as fill the SMs, by their number on a B200 (the
+// caller's scratch goes by it, whichever device is current).
+RowsPlan rows_plan(int vh, int rows, long long pages, bool join) {
+  RowsPlan p = {};
+  p.rg = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  p.dg = 1;
+  p.clusters = 1;
+  const int most = pages < MAX_SPLITS ? (int)pages : MAX_SPLITS;
+  p.splits = 1;
+  if (join) {
+    // as many splits as leave all clusters resident
+    for (p.splits = most; p.splits > 1 && rows_resident(p) < vh; --p.splits) {}
+    if (p.rg == 1 && p.splits == MAX_SPLITS && pages >= 3 * MAX_SPLITS) {
+      // few heads and long windows: three groups of warps, a tile each, on an SM of their own
+      p.dg = 3;
+      if (rows_resident(p) < vh) p.dg = 1;
+    }
+  } else {
+    const int per_sm = p.rg == 4 ? 1 : 2;
+    p.splits = most < 4 ? most : 4;
+    long long n = (long long)per_sm * 132 / ((long long)vh * p.splits);
+    if (n > pages / p.splits) n = pages / p.splits;
+    p.clusters = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+  }
+  rows_sizes(p, rows, (pages + (long long)p.splits * p.clusters - 1) / ((long long)p.splits * p.clusters));
+  return p;
 }
 
 int rows_launch(const RowsPlan& p, RowsArgs& a, int vh, const char* who, cudaStream_t stream) {
@@ -472,10 +473,11 @@ int rows_launch(const RowsPlan& p, RowsArgs& a, int vh, const char* who, cudaStr
   if (!status) { q_set_error("%s: could not locate the device status word", who); return Q_ERR_CUDA; }
   a.share = p.share;
   a.stages = p.stages;
-  if (p.nt == 4) Q_CHECK_CUDA((rows_go<4, 1>(p, a, vh, status, stream)));
-  else if (p.nt == 2) Q_CHECK_CUDA((rows_go<2, 1>(p, a, vh, status, stream)));
-  else if (p.groups == 3) Q_CHECK_CUDA((rows_go<1, 3>(p, a, vh, status, stream)));
-  else Q_CHECK_CUDA((rows_go<1, 1>(p, a, vh, status, stream)));
+  static size_t done[4][64] = {{0}};
+  const rows_kernel k = rows_form(p);
+  Q_CHECK_CUDA(q_ensure_smem(k, p.smem, done[p.rg == 4 ? 3 : p.rg == 2 ? 2 : p.dg == 3 ? 1 : 0]));
+  Q_CHECK_CUDA(q_launch_cluster(k, dim3(p.splits * p.clusters, vh), dim3((4 * p.rg * p.dg + 1) * 32), p.smem, stream,
+                                (unsigned)p.splits, a, status));
   return Q_OK;
 }
 
@@ -550,8 +552,7 @@ SharedPlan shared_plan(int batch, int T, int n_q_heads, int nkv, long long prefi
     s.plan = rows_plan(nkv, s.rows, prefix_pages, false);
     s.parts = s.plan.clusters;
   } else {
-    int sms = q_sm_count();
-    if (sms <= 0) sms = 148;
+    constexpr int sms = 148;
     const int tokens = 128 / G, tiles = (batch * T + tokens - 1) / tokens, blocks = tiles == 1 ? 1 : (tiles + 1) / 2;
     long long n = sms / ((long long)nkv * blocks);
     if (n > (prefix_pages + 1) / 2) n = (prefix_pages + 1) / 2;
