@@ -30,6 +30,10 @@
 // 64 rows x 64 dims lands as rows of 128 bytes, and the pages' own chunk swizzle (chunk ^ row & 7)
 // is then the 128-byte swizzle the MMA descriptors name. Every wait is bounded.
 //
+// DEEP (one tile per CTA): the other half of tensor memory holds a second set of scores, so that those of the next
+// key tile are there when the softmax of this one ends, and the tensor cores work under it; queries of the next item
+// lie in the second tile's place. A step then waits for the softmax alone, not for the chain.
+//
 // Three forms (FORM) walk other keys with the same pipeline: CAUSAL (the prompt), WINDOW (the prompt under a
 // sliding window with sinks: of the key tiles only those that hold a key some row of the item sees), PARTS (many
 // rows over one range of keys that all of them see, cut into key splits whose m, l and O are left in 32 bits).
@@ -51,7 +55,7 @@ constexpr uint32_t AP_BARS = AP_V + 2 * AP_TILE;           // 192 KB in
 constexpr uint32_t AP_RED = AP_BARS + 24 * 8 + 16;         // row exchange: [3][2 tiles x 2 or 4 parts][128] floats
 constexpr size_t AP_SMEM = 1024 + AP_RED + 3 * 2 * 2 * 128 * 4;
 
-enum { B_QF = 0, B_QE = 2, B_KF = 4, B_KE = 6, B_VF = 8, B_VE = 10, B_SF = 12, B_P = 14, B_OF = 18, B_OE = 20 };
+enum { B_QF = 0, B_QE = 2, B_KF = 4, B_KE = 6, B_VF = 8, B_VE = 10, B_SF = 12, B_P = 14, B_OF = 18, B_OE = 20, B_PV = 22 };
 
 struct AttnShape {
   int batch, T, G, gshift, nq, nkv, pages_per_seq;
@@ -146,6 +150,25 @@ __device__ __forceinline__ int item_of(int round) {
   return round * g + ((round & 1) ? g - 1 - (int)blockIdx.x : (int)blockIdx.x);
 }
 
+// The key tiles of a CTA's items in order.
+template <int FORM>
+struct Walk {
+  Item it;
+  int r, j;          // round of the item, tile of the item
+  bool more;         // there is a tile here
+  __device__ __forceinline__ void seek(const AttnShape& sh, int items, int pos, const int32_t* pos_ptr) {
+    for (; r * (int)gridDim.x < items; ++r) {
+      const int w = item_of(r);
+      if (w < items) { it = item_of_form<FORM>(sh, w, pos, pos_ptr); j = 0; more = true; return; }
+    }
+    more = false;
+  }
+  __device__ __forceinline__ void next(const AttnShape& sh, int items, int pos, const int32_t* pos_ptr) {
+    if (++j < it.n) return;
+    ++r;
+    seek(sh, items, pos, pos_ptr);
+  }
+};
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w,
                                             uint32_t bar) {
   asm volatile(
@@ -195,6 +218,8 @@ __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&r)[16])
       : "memory");
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// The lowest n bits (none for n <= 0, all from 32 on).
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 // Two fp32 lanes per instruction, each rounded like the scalar one; and the largest of three.
 __device__ __forceinline__ unsigned long long pair2(float a, float b) {
   unsigned long long r;
@@ -225,11 +250,12 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-template <int TILES, int FORM>
+template <int TILES, int FORM, bool DEEP>
 __global__ void __launch_bounds__(AP_THREADS, 1)
 k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
               const __grid_constant__ CUtensorMap vmap, const int32_t* __restrict__ block_table,
               const int32_t* __restrict__ pos_ptr, bf16* __restrict__ out, AttnShape sh, int* status) {
+  static_assert(!DEEP || (TILES == 1 && FORM != CAUSAL), "one tile of the other forms");
   constexpr int WARPS = TILES == 2 ? 8 : 16;               // softmax warps of a query tile
   constexpr int PER_ROW = WARPS / 4, COLS = 128 / PER_ROW; // threads of a row, scores (and dims of O) of each
   extern __shared__ unsigned char smem_raw[];
@@ -295,6 +321,58 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
       uint32_t nitems = 0;
       bool ok = true;
       auto fail = [&]() { atomicExch(status, 7); *abort_flag = 1; ok = false; };
+      if constexpr (DEEP) {
+        // keys run one tile ahead of values: their place is free as soon as their scores are
+        Walk<FORM> k, v;
+        k.r = v.r = 0;
+        k.seek(sh, items, pos, pos_ptr);
+        v = k;
+        uint32_t ksteps = 0, vsteps = 0;
+        auto load = [&](const Walk<FORM>& at, bool values, uint32_t n) {
+          const int key_base = key_base_of<FORM>(at.it, at.j), first = key_base / Q_PAGE_TOKENS;
+          const uint32_t live = live_steps<FORM>(sh, at.it, key_base);
+          const int32_t* table = block_table + (size_t)at.it.b * sh.pages_per_seq;
+          const int p0 = live & 0x0fu ? 0 : 1, np = live & 0xf0u ? 2 : 1;      // a page that nobody sees is not read
+          const int page0 = p0 == 0 ? __ldcg(table + first) : 0, page1 = np == 2 ? __ldcg(table + first + 1) : 0;
+          const int s = n & 1;
+          if (!mbar_wait(bar(values ? B_VE : B_KE, s), ((n >> 1) & 1) ^ 1, abort_flag)) { fail(); return; }
+          const uint32_t full = bar(values ? B_VF : B_KF, s), dst = base + (values ? AP_V : AP_K) + s * AP_TILE;
+          mbar_expect_tx(full, (uint32_t)(np - p0) * AP_HALF);
+          for (int p = p0; p < np; ++p)
+            for (int h = 0; h < 2; ++h)
+              tma_load_4d(dst + h * AP_HALF + p * (AP_HALF / 2), values ? &vmap : &kmap, 0, h, 0,
+                          (p ? page1 : page0) * sh.nkv + at.it.kh, full);
+        };
+        while (ok && v.more) {
+          if (k.more) {
+            if (k.j == 0) {
+              const int slot = nitems & 1;
+              if (!mbar_wait(bar(B_QE, slot), ((nitems >> 1) & 1) ^ 1, abort_flag)) { fail(); break; }
+              mbar_expect_tx(bar(B_QF, slot), (uint32_t)(sh.tokens * sh.G) * 256u);
+              for (int h = 0; h < 2; ++h)
+                tma_load_3d(base + AP_Q + slot * AP_TILE + h * AP_HALF, &qmap, 64 * h, k.it.kh * sh.G,
+                            k.it.b * sh.T + k.it.q0, bar(B_QF, slot));
+              ++nitems;
+            }
+            load(k, false, ksteps);
+            if (!ok) break;
+            ++ksteps;
+            k.next(sh, items, pos, pos_ptr);
+          }
+          if (ksteps < 2 && k.more) continue;              // (the first two tiles' keys go first)
+          load(v, true, vsteps);
+          if (!ok) break;
+          ++vsteps;
+          v.next(sh, items, pos, pos_ptr);
+        }
+        // copies in flight must land before the CTA may leave
+        for (uint32_t i = 0; i < 2; ++i) {
+          if (nitems > i) mbar_wait_plain(bar(B_QF, (nitems - 1 - i) & 1), ((nitems - 1 - i) >> 1) & 1);
+          if (ksteps > i) mbar_wait_plain(bar(B_KF, (ksteps - 1 - i) & 1), ((ksteps - 1 - i) >> 1) & 1);
+          if (vsteps > i) mbar_wait_plain(bar(B_VF, (vsteps - 1 - i) & 1), ((vsteps - 1 - i) >> 1) & 1);
+        }
+        nitems = 0;
+      } else
       for (int r = 0; ok && r * (int)gridDim.x < items; ++r) {
         const int w = item_of(r);
         if (w >= items) continue;
@@ -380,9 +458,79 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
         }
         tc_commit(bar(B_SF, i));
       };
+      if constexpr (DEEP) {
+        Walk<FORM> s, v;                                   // tiles of the next scores and the next products
+        s.r = 0;
+        s.seek(sh, items, pos, pos_ptr);
+        v = s;
+        uint32_t qitems = 0;                               // items whose queries have been waited for
+        auto ahead = [&]() {                               // scores of the tile at s into the buffer of its parity
+          if (s.j == 0) {
+            if (!wait(bar(B_QF, qitems & 1), (qitems >> 1) & 1)) return;
+            ++qitems;
+          }
+          if (!wait(bar(B_KF, kstep & 1), (kstep >> 1) & 1)) return;
+          const uint32_t buf = kstep & 1, slot = (qitems - 1) & 1;
+          const uint64_t a = q_desc + (uint64_t)(slot * (AP_TILE >> 4)), b = k_desc + (uint64_t)(buf * (AP_TILE >> 4));
+          const bool last = s.j + 1 == s.it.n;
+          if (elect_one()) {
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) {
+              const uint32_t off = (uint32_t)(ks >> 2) * (AP_HALF >> 4) + (ks & 3) * 2;
+              tc_mma(tmem + 128u * buf, a + off, b + off, idesc_s, ks ? 1u : 0u);
+            }
+            tc_commit(bar(B_SF, buf));
+            tc_commit(bar(B_KE, buf));
+            if (last) tc_commit(bar(B_QE, slot));
+          }
+          __syncwarp();
+          ++kstep;
+          s.next(sh, items, pos, pos_ptr);
+        };
+        for (int i = 0; i < 2 && ok && s.more; ++i) ahead();
+        while (ok && v.more) {
+          const uint32_t buf = vstep & 1, parity = (vstep >> 1) & 1;
+          const int key_base = key_base_of<FORM>(v.it, v.j);
+          const bool last = v.j + 1 == v.it.n;
+          const uint32_t live = live_steps<FORM>(sh, v.it, key_base);
+          if (!wait(bar(B_VF, buf), parity)) break;
+          if (v.j == 0 && !wait(bar(B_OE, 0), (nitems & 1) ^ 1)) break;
+          if (!wait(bar(B_P, 2 * buf), parity) || !wait(bar(B_P, 2 * buf + 1), parity)) break;
+          const bool first = v.j == 0;
+          v.next(sh, items, pos, pos_ptr);
+          if (elect_one()) {
+            const uint64_t b = v_desc + (uint64_t)(buf * (AP_TILE >> 4));
+            if (live == 0xffu) {
+#pragma unroll
+              for (int ks = 0; ks < 8; ++ks)
+                tc_mma_ta(tmem + 256u, tmem + 128u * buf + 8u * ks, b + (uint64_t)(ks * (2048 >> 4)), idesc_pv, (!first || ks) ? 1u : 0u);
+            } else {
+              uint32_t sum = first ? 0u : 1u;
+#pragma unroll 1
+              for (int ks = 0; ks < 8; ++ks) {
+                if (!((live >> ks) & 1u)) continue;
+                tc_mma_ta(tmem + 256u, tmem + 128u * buf + 8u * ks, b + (uint64_t)(ks * (2048 >> 4)), idesc_pv, sum);
+                sum = 1u;
+              }
+            }
+            // (nothing after the last tile's: nobody waits for it any more, and the arrival could find that the CTA has left)
+            if (v.more) {
+              tc_commit(bar(B_VE, buf));
+              tc_commit(bar(B_PV, 0));
+            }
+            if (last) tc_commit(bar(B_OF, 0));
+          }
+          __syncwarp();
+          ++vstep;
+          if (last) ++nitems;
+          if (s.more) ahead();
+        }
+        ok = false;                                        // (nothing is left)
+      }
       int r = 0;
-      if (idle) ok = false;                                // (nothing is waited for)
-      Item cur = item_of_form<FORM>(sh, idle ? 0 : item_of(0), idle ? 1 : pos, pos_ptr);  // the grid has at most one CTA per item
+      if (DEEP || idle) ok = false;                        // (nothing is waited for)
+      Item cur = {};
+      if (ok) cur = item_of_form<FORM>(sh, item_of(0), pos, pos_ptr);      // the grid has at most one CTA per item
       for (int i = 0; i < TILES && ok; ++i) {
         if (!wait(bar(B_QF, i), 0) || (i == 0 && !wait(bar(B_KF, 0), 0))) break;
         scores(i);
@@ -468,7 +616,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
     float* red = reinterpret_cast<float*>(smem + AP_RED) + i * 256;        // [buffer * 512 + part * 128 + row]
     auto tile_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + i), "n"(WARPS * 32) : "memory"); };
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + 128u * i + (uint32_t)(COLS * part), p_addr = tmem + lanes + 128u * i + (uint32_t)(COLS / 2 * part);
+    uint32_t s_addr = tmem + lanes + 128u * i + (uint32_t)(COLS * part), p_addr = tmem + lanes + 128u * i + (uint32_t)(COLS / 2 * part);
     const uint32_t o_addr = tmem + lanes + 256u + 128u * i + (uint32_t)(COLS * part);
     // A scale that is not positive (the maximum would sit elsewhere) is multiplied in first.
     const bool plain = sh.scale_log2 > 0.f;
@@ -510,7 +658,12 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
       }
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < it.n; ++j, ++step) {
-        wait(bar(B_SF, i), step & 1);
+        const uint32_t buf = DEEP ? step & 1 : (uint32_t)i;
+        if (DEEP) {
+          s_addr = tmem + lanes + 128u * buf + (uint32_t)(COLS * part);
+          p_addr = tmem + lanes + 128u * buf + (uint32_t)(COLS / 2 * part);
+        }
+        wait(bar(B_SF, buf), DEEP ? (step >> 1) & 1 : step & 1);
         float v[COLS];
         if constexpr (TILES == 2) {
           tc_ld32(s_addr, v);
@@ -532,10 +685,14 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
         }
         if (FORM == WINDOW) {
           if (key_base + AP_KEYS > free_keys || (key_base < free_from && key_base + AP_KEYS > sh.sinks)) {
-            const int vis = limit - key_base - COLS * part, from = low - key_base - COLS * part,
-                      sunk = sh.sinks - key_base - COLS * part;
+            // a bit per score: with three comparisons each a tile took 1900 cycles more, of 3400
 #pragma unroll
-            for (int k = 0; k < COLS; ++k) v[k] = k < vis && (k >= from || k < sunk) ? v[k] : -INFINITY;
+            for (int h = 0; h < COLS; h += 32) {
+              const int at = key_base + COLS * part + h;
+              const uint32_t seen = below(limit - at) & (~below(low - at) | below(sh.sinks - at));
+#pragma unroll
+              for (int k = 0; k < 32; ++k) v[h + k] = seen & (1u << k) ? v[h + k] : -INFINITY;
+            }
           }
         } else if (key_base + AP_KEYS > free_keys) {
           const int vis = limit - key_base - COLS * part;
@@ -590,8 +747,13 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
         if (j == 0) {
           m = m_tile;
         } else {
-          if (__any_sync(0xffffffffu, m_tile > m)) {
-            // the products up to the tile before are complete: this tile's scores came after them
+          // (the other forms let it grow by 2^4 first: over few tiles some row of a warp has a new maximum in nearly
+          // each, and reading and writing O took a quarter of a step. P is then at most 16, as exact in bf16 as up to
+          // 1; only a row's largest is no longer exactly 1.)
+          if (__any_sync(0xffffffffu, FORM == CAUSAL ? m_tile > m : (m_tile - m) * c > 4.f)) {
+            // the products up to the tile before are complete: this tile's scores came after them (DEEP: after those
+            // of the tile before that, so that the parity of the last ones names them)
+            if (DEEP) wait(bar(B_PV, 0), (step - 1) & 1);
             const float m_new = fmaxf(m, m_tile);
             const float f = m_new == m ? 1.f : ex2((m - m_new) * c);
             l *= f;
@@ -628,7 +790,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_P, 2 * i + part / (PER_ROW / 2)));
+        if (lane == 0) mbar_arrive(bar(B_P, 2 * buf + part / (PER_ROW / 2)));
         __syncwarp();
         float s_lo, s_hi;
         unpair2(add2(sum[0], sum[1]), s_lo, s_hi);
@@ -776,7 +938,7 @@ int prompt_launch(const char* who, AttnShape& sh, const void* d_q, const q_kv_la
     if (rc) return rc;
   }
   static size_t done[2][64] = {{0}};
-  auto kern = sh.tiles == 2 ? k_attn_prompt<2, FORM> : k_attn_prompt<1, FORM>;
+  auto kern = sh.tiles == 2 ? k_attn_prompt<2, FORM, false> : k_attn_prompt<1, FORM, FORM != CAUSAL>;
   Q_CHECK_CUDA(q_ensure_smem(kern, AP_SMEM, done[sh.tiles - 1]));
   const int grid = sh.items < sms ? sh.items : sms;
   Q_CHECK_CUDA(q_launch(kern, dim3(grid), dim3(AP_THREADS), AP_SMEM, (cudaStream_t)stream, qmap, kmap, vmap,
