@@ -323,10 +323,10 @@ k_attn_rows(RowsArgs a, int* status) {
         Lsum += wt * mml[(w * R + r) * 2 + 1];
         O += wt * mo[(w * R + r) * ROW_LD + d];
       }
-      // to the CTA that joins this (row, dim): slot `rank` of its receive area
-      const int v = r * 128 + d, owner = v / a.share;
+      // to the CTA that joins this row: slot `rank` of its receive area
+      const int owner = r % S, at = r / S;
       asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote_addr(smem_u32(recv), owner) +
-                   (uint32_t)(rank * a.share + (v - owner * a.share)) * 4u), "f"(O) : "memory");
+                   (uint32_t)(rank * a.share + at * 128 + d) * 4u), "f"(O) : "memory");
       if (d < S)           // the row's maximum and sum go to every CTA of the cluster (thread d -> CTA d)
         asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(remote_addr(smem_u32(recv), d) +
                      (uint32_t)(S * a.share + (rank * R + r) * 2) * 4u), "f"(Mx), "f"(Lsum) : "memory");
@@ -338,17 +338,24 @@ k_attn_rows(RowsArgs a, int* status) {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (a.early) pdl_wait();       // the prefix's partial rows are complete
+  // a warp joins a row: rank, rank + S, ..
   const float* rml = recv + S * a.share;
-  const int total = R * 128, own0 = rank * a.share;
   const int psplits = a.parts.splits > 0 && !a.write_parts ? parts_used(a.parts) : 0;
-  for (int c = warp * 32; c < a.share && own0 + c < total; c += DT) {
-    const int r = (own0 + c) >> 7, d = ((own0 + c) & 127) + lane;
+  for (int at = warp; rank + at * S < R; at += DC + 1) {
+    const int r = rank + at * S;
     const int t = r / a.G, hg = r - t * a.G;
+    const size_t prow = (size_t)(b * a.T + t) * a.G + hg;
+    // all of the prefix's first parts are asked for at once, with their maxima and sums
+    constexpr int AHEAD = RG == 1 ? 16 : 8;
+    float4 o[AHEAD];
+    if (psplits > 0)
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+        o[j] = j < psplits ? __ldcg(reinterpret_cast<const float4*>(a.parts.o + a.parts.row(j, kh, prow) * 128) + lane)
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
     float2 ml = make_float2(-INFINITY, 0.f);
     if (lane < S) ml = *reinterpret_cast<const float2*>(rml + (lane * R + r) * 2);
-    // the prefix's parts of this row: lane and lane + 32
-    float2 pml[2] = {make_float2(-INFINITY, 0.f), make_float2(-INFINITY, 0.f)};
-    const size_t prow = (size_t)(b * a.T + t) * a.G + hg;
+    float2 pml[2] = {make_float2(-INFINITY, 0.f), make_float2(-INFINITY, 0.f)};      // parts lane and lane + 32
 #pragma unroll
     for (int e = 0; e < 2; ++e)
       if (lane + 32 * e < psplits) pml[e] = __ldcg(a.parts.ml + a.parts.row(lane + 32 * e, kh, prow));
@@ -361,26 +368,34 @@ k_attn_rows(RowsArgs a, int* status) {
     float l = (ml.y == ml.y ? w * ml.y : ml.y) + (pml[0].y == pml[0].y ? pw[0] * pml[0].y : pml[0].y) +
               (pml[1].y == pml[1].y ? pw[1] * pml[1].y : pml[1].y);
     l = warp_sum(l);
-    float O = 0.f;
-    for (int s = 0; s < S; ++s) O += __shfl_sync(0xffffffffu, w, s) * recv[s * a.share + c + lane];
-    for (int s0 = 0; s0 < psplits; s0 += 8) {
-      float o[8];
+    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float f, float4 x) { O.x += f * x.x; O.y += f * x.y; O.z += f * x.z; O.w += f * x.w; };
+    for (int s = 0; s < S; ++s)
+      add(__shfl_sync(0xffffffffu, w, s), *reinterpret_cast<const float4*>(recv + s * a.share + at * 128 + 4 * lane));
+    if (psplits > 0)
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        o[j] = s0 + j < psplits ? __ldcg(a.parts.o + a.parts.row(s0 + j, kh, prow) * 128 + d) : 0.f;
+      for (int j = 0; j < AHEAD; ++j) add(__shfl_sync(0xffffffffu, pw[0], j), o[j]);
+    for (int s0 = AHEAD; s0 < psplits; s0 += AHEAD) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < AHEAD; ++j)
+        o[j] = s0 + j < psplits ? __ldcg(reinterpret_cast<const float4*>(a.parts.o + a.parts.row(s0 + j, kh, prow) * 128) + lane)
+                                : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
         const float lo = __shfl_sync(0xffffffffu, pw[0], (s0 + j) & 31), hi = __shfl_sync(0xffffffffu, pw[1], (s0 + j) & 31);
-        O += (s0 + j < 32 ? lo : hi) * o[j];
+        add(s0 + j < 32 ? lo : hi, o[j]);
       }
     }
     if (a.write_parts) {
       const size_t row = a.parts.row(blockIdx.x / S, kh, prow);
-      a.parts.o[row * 128 + d] = O;
-      if (d == 0) a.parts.ml[row] = make_float2(Mx, l);
+      *(reinterpret_cast<float4*>(a.parts.o + row * 128) + lane) = O;
+      if (lane == 0) a.parts.ml[row] = make_float2(Mx, l);
     } else {
-      const float res = l > 0.f ? O / l : l == 0.f ? 0.f : l;
-      a.out[((size_t)(b * a.T + t) * a.nq + kh * a.G + hg) * 128 + d] = __float2bfloat16_rn(res);
+      const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+      uint2 packed;
+      packed.x = pack_bf16(O.x * inv, O.y * inv);
+      packed.y = pack_bf16(O.z * inv, O.w * inv);
+      *reinterpret_cast<uint2*>(a.out + ((size_t)(b * a.T + t) * a.nq + kh * a.G + hg) * 128 + 4 * lane) = packed;
     }
   }
 }
@@ -406,7 +421,7 @@ void rows_sizes(RowsPlan& p, int rows, long long each) {
   if (each < p.stages) p.stages = each < 1 ? 1 : (int)each;
   if (p.dg == 3) p.stages = 3;                    // a stage always belongs to the same group, which tracks its parity
   if (p.stages < need) p.stages = need;
-  p.share = ((rows * 128 + p.splits - 1) / p.splits + 31) / 32 * 32;
+  p.share = (rows + p.splits - 1) / p.splits * 128;
   p.smem = rows_smem(p, rows);
 }
 
@@ -493,7 +508,7 @@ int check_rows(const char* who, const void* d_q, const q_kv_layout_t* kv, const 
   Q_CHECK_ARG((long long)batch * nkv <= 65535, "%s: too many (sequence, kv head) pairs", who);
   Q_CHECK_ARG(kv->pages_per_seq <= (1 << 24), "%s: too many pages per sequence", who);
   Q_CHECK_ALIGN(d_q, 16, who); Q_CHECK_ALIGN(kv->d_kpool, 16, who); Q_CHECK_ALIGN(kv->d_vpool, 16, who);
-  Q_CHECK_ALIGN(d_out, 2, who); Q_CHECK_ALIGN(d_pos, 4, who); Q_CHECK_ALIGN(kv->d_block_table, 4, who);
+  Q_CHECK_ALIGN(d_out, 8, who); Q_CHECK_ALIGN(d_pos, 4, who); Q_CHECK_ALIGN(kv->d_block_table, 4, who);
   return Q_OK;
 }
 

@@ -33,11 +33,14 @@ def _stream() -> C.c_void_p:
 def _call(device: torch.device, fn, *args) -> None:
     """fn(*args, stream) on the current stream of `device`, whichever device is current. (The Stream object that
     torch.cuda.current_stream() makes costs 3.3 us, the context 1.4, of a call's 16 - 18.)"""
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)))
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc)
 
 
 def _ptr(t: torch.Tensor | None) -> C.c_void_p:
@@ -266,7 +269,10 @@ class PagedKV:
         if (block_table.shape != (batch, self.pages_per_seq) or block_table.dtype != torch.int32
                 or not block_table.is_contiguous()):
             raise ValueError("block table must be contiguous int32 [batch, pages_per_seq]")
+        if block_table.device != self.k.device:
+            raise ValueError("block table and pages are on different devices")
         self.block_table = block_table
+        self.device = self.k.device
         self.layout = KVLayout(self.k.data_ptr(), self.v.data_ptr(), block_table.data_ptr(),
                                self.pages_per_seq, n_kv_heads)
 
@@ -395,18 +401,18 @@ def prompt_attention(query: torch.Tensor, cache: PagedKV, position: torch.Tensor
 def _positions(position: torch.Tensor, batch: int, device) -> int:
     """Checks an int32 CUDA position tensor of shape [1] (all sequences) or [batch]; whether it has one per
     sequence."""
-    if (tuple(position.shape) not in ((1,), (batch,)) or position.dtype != torch.int32 or position.device != device
-            or not position.is_contiguous()):
+    n = position.shape[0] if position.ndim == 1 else 0
+    if (n != 1 and n != batch) or n == 0 or position.dtype != torch.int32 or position.device != device or (
+            n > 1 and not position.is_contiguous()):
         raise ValueError("position must be a contiguous int32 tensor of shape [1] or [batch] on the query's device")
-    return int(position.shape[0] == batch)
+    return int(n == batch)
 
 
-def _paged_query(query: torch.Tensor, cache: PagedKV, rows: int, heads: int | None) -> None:
-    if (query.ndim != 3 or query.shape[0] != rows or query.shape[2] != HEAD_DIM
-            or (heads is not None and query.shape[1] != heads)
-            or query.dtype != torch.bfloat16 or not query.is_cuda or not query.is_contiguous()):
+def _paged_query(query: torch.Tensor, rows: int, heads: int, device) -> None:
+    if (query.shape != (rows, heads, HEAD_DIM) or query.dtype != torch.bfloat16 or not query.is_cuda
+            or not query.is_contiguous()):
         raise ValueError("expected contiguous BF16 CUDA Q [batch*T, Hq, 128]")
-    if cache.k.device != query.device or cache.block_table.device != query.device:
+    if query.device != device:
         raise ValueError("query and cache are on different devices")
 
 
@@ -430,12 +436,13 @@ class WindowAttention:
 
     def run(self, query, cache: PagedKV, position, scale) -> torch.Tensor:
         """query [batch*T, Hq, 128] -> [batch*T, Hq*128]."""
-        _paged_query(query, cache, self.batch * self.T, self.hq)
+        device = cache.device
+        _paged_query(query, self.batch * self.T, self.hq, device)
         if cache.batch != self.batch or cache.n_kv != self.hk or cache.capacity < self.capacity:
             raise ValueError("cache does not match this attention instance")
-        each = _positions(position, self.batch, query.device)
-        out = torch.empty((self.batch * self.T, self.hq * HEAD_DIM), dtype=torch.bfloat16, device=query.device)
-        _call(query.device, lib.q_attention_window, query.data_ptr(), C.byref(cache.layout), position.data_ptr(), each,
+        each = _positions(position, self.batch, device)
+        out = torch.empty((self.batch * self.T, self.hq * HEAD_DIM), dtype=torch.bfloat16, device=device)
+        _call(device, lib.q_attention_window, query.data_ptr(), C.byref(cache.layout), position.data_ptr(), each,
               out.data_ptr(), self.batch, self.T, self.hq, self.window, self.sinks, scale)
         return out
 
@@ -447,11 +454,13 @@ def window_prompt_attention(query: torch.Tensor, cache: PagedKV, position: torch
     T = int(tokens_per_seq)
     if T < 1:
         raise ValueError("at least one token per sequence")
-    _paged_query(query, cache, cache.batch * T, None)
+    if query.ndim != 3:
+        raise ValueError("expected contiguous BF16 CUDA Q [batch*T, Hq, 128]")
+    hq = query.shape[1]
+    _paged_query(query, cache.batch * T, hq, cache.device)
     if not 1 <= window < 2 ** 31 or not 0 <= sinks < 2 ** 31:
         raise ValueError("the window must hold at least one key, and sinks cannot be negative")
     each = _positions(position, cache.batch, query.device)
-    hq = query.shape[1]
     out = torch.empty((cache.batch * T, hq * HEAD_DIM), dtype=torch.bfloat16, device=query.device)
     _call(query.device, lib.q_attention_window_prefill, query.data_ptr(), C.byref(cache.layout), position.data_ptr(),
           each, out.data_ptr(), cache.batch, T, hq, int(window), int(sinks), scale)
@@ -478,23 +487,23 @@ class SharedPrefixAttention:
 
     def run(self, query, prefix: PagedKV, prefix_length, cache: PagedKV, position, scale) -> torch.Tensor:
         """query [batch*T, Hq, 128] -> [batch*T, Hq*128]."""
-        _paged_query(query, cache, self.batch * self.T, self.hq)
-        _paged_query(query, prefix, self.batch * self.T, self.hq)
+        device = cache.device
+        _paged_query(query, self.batch * self.T, self.hq, device)
         if cache.batch != self.batch or cache.n_kv != self.hk or cache.capacity < self.capacity:
             raise ValueError("cache does not match this attention instance")
         if prefix.batch != 1 or prefix.n_kv != self.hk or prefix.capacity < self.prefix_capacity:
             raise ValueError("the prefix must be one sequence that matches this attention instance")
-        if (tuple(prefix_length.shape) != (1,) or prefix_length.dtype != torch.int32
-                or prefix_length.device != query.device):
-            raise ValueError("prefix_length must be an int32 tensor of shape [1] on the query's device")
-        each = _positions(position, self.batch, query.device)
+        if (prefix_length.shape != (1,) or prefix_length.dtype != torch.int32 or prefix_length.device != device
+                or prefix.device != device):
+            raise ValueError("prefix_length must be an int32 tensor of shape [1], it and the prefix on the query's device")
+        each = _positions(position, self.batch, device)
         if prefix.pages_per_seq != self._planned:
             self._scratch = lib.q_attention_shared_scratch_bytes(self.batch, self.T, self.hq, self.hk,
                                                                  prefix.pages_per_seq)
             self._planned = prefix.pages_per_seq
-        out = torch.empty((self.batch * self.T, self.hq * HEAD_DIM), dtype=torch.bfloat16, device=query.device)
-        scratch = torch.empty(max(16, self._scratch), dtype=torch.uint8, device=query.device)
-        _call(query.device, lib.q_attention_shared, query.data_ptr(), C.byref(prefix.layout), prefix_length.data_ptr(),
+        out = torch.empty((self.batch * self.T, self.hq * HEAD_DIM), dtype=torch.bfloat16, device=device)
+        scratch = torch.empty(self._scratch or 16, dtype=torch.uint8, device=device)
+        _call(device, lib.q_attention_shared, query.data_ptr(), C.byref(prefix.layout), prefix_length.data_ptr(),
               C.byref(cache.layout), position.data_ptr(), each, scratch.data_ptr(), out.data_ptr(), self.batch, self.T,
               self.hq, scale)
         return out
@@ -544,7 +553,7 @@ def _setting(value, rows: int, device, dtype, what: str):
     """(number, pointer): a number for all rows, or a tensor with one per row."""
     if not isinstance(value, torch.Tensor):
         return value, 0
-    if tuple(value.shape) != (rows,) or value.dtype != dtype or value.device != device or not value.is_contiguous():
+    if value.shape != (rows,) or value.dtype != dtype or value.device != device or not value.is_contiguous():
         raise ValueError(f"{what} must be a number or a contiguous {dtype} tensor [rows] on the logits' device")
     return 0, value.data_ptr()
 
@@ -558,13 +567,13 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     draws from the same logits); uniform: FP32 [rows] in [0, 1). Every setting is a
     number, or a tensor with one per row (FP32; top_k int32). temperature 0 is greedy. Returns (tokens int64 [rows],
     logprobs FP32 [rows]): -1 and -inf for a row without a finite logit."""
-    if (logits.ndim != 2 or not logits.is_cuda or logits.dtype not in (torch.bfloat16, torch.float32)
-            or logits.shape[0] < 1 or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1)):
+    fp32 = logits.dtype == torch.float32
+    if (logits.ndim != 2 or not logits.is_cuda or not (fp32 or logits.dtype == torch.bfloat16) or logits.numel() < 1
+            or (logits.shape[1] > 1 and logits.stride(1) != 1)):
         raise ValueError("logits must be a BF16 or FP32 CUDA [rows, vocab] tensor with adjacent columns")
     rows, vocab = logits.shape
     dev = logits.device
-    if (tuple(uniform.shape) != (rows,) or uniform.dtype != torch.float32 or uniform.device != dev
-            or not uniform.is_contiguous()):
+    if uniform.shape != (rows,) or uniform.dtype != torch.float32 or uniform.device != dev or not uniform.is_contiguous():
         raise ValueError("uniform must be a contiguous FP32 tensor [rows] on the logits' device")
     t, dt = _setting(temperature, rows, dev, torch.float32, "temperature")
     k, dk = _setting(top_k, rows, dev, torch.int32, "top_k")
@@ -575,8 +584,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     settings = _lib.Sampling(t, int(k), p, m, dt, dk, dp, dm)
     tokens = torch.empty(rows, dtype=torch.int64, device=dev)
     logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
-    _call(dev, lib.q_sample_tokens, logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0),
-          uniform.data_ptr(), C.byref(settings), tokens.data_ptr(), logprobs.data_ptr(), rows, vocab)
+    _call(dev, lib.q_sample_tokens, logits.data_ptr(), fp32, logits.stride(0), uniform.data_ptr(), C.byref(settings),
+          tokens.data_ptr(), logprobs.data_ptr(), rows, vocab)
     return tokens, logprobs
 
 
