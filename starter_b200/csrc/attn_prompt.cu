@@ -747,10 +747,11 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
         if (j == 0) {
           m = m_tile;
         } else {
-          // (the other forms let it grow by 2^4 first: over few tiles some row of a warp has a new maximum in nearly
-          // each, and reading and writing O took a quarter of a step. P is then at most 16, as exact in bf16 as up to
-          // 1; only a row's largest is no longer exactly 1.)
-          if (__any_sync(0xffffffffu, FORM == CAUSAL ? m_tile > m : (m_tile - m) * c > 4.f)) {
+          // (the other forms let it grow by 2^8 first: over few tiles some row of a warp has a new maximum in nearly
+          // each, and reading and writing O took a quarter of a step. P is then at most 256, as exact in bf16 as up to
+          // 1; only a row's largest is no longer exactly 1. A prompt of 7000 tokens under a window of 1024, at once / after
+          // 2^8, us: 174 / 163; of 5000 under 4096: 221 / 207.)
+          if (__any_sync(0xffffffffu, FORM == CAUSAL ? m_tile > m : (m_tile - m) * c > 8.f)) {
             // the products up to the tile before are complete: this tile's scores came after them (DEEP: after those
             // of the tile before that, so that the parity of the last ones names them)
             if (DEEP) wait(bar(B_PV, 0), (step - 1) & 1);

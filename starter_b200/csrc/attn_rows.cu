@@ -100,7 +100,6 @@ template <int RG, int DG, int BLOCKS>
 __global__ void __launch_bounds__((4 * RG * DG + 1) * 32, BLOCKS)
 k_attn_rows(RowsArgs a, int* status) {
   constexpr int DC = 4 * RG * DG;                  // consumer warps
-  constexpr int DT = (DC + 1) * 32;
   constexpr int SETS = 4;                          // accumulators of Q K^T: an MMA's result is ~280 cycles away
   extern __shared__ __align__(1024) unsigned char smem[];
   const int NS = a.stages;
