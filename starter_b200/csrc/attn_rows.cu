@@ -345,7 +345,7 @@ k_attn_rows(RowsArgs a, int* status) {
     const int t = r / a.G, hg = r - t * a.G;
     const size_t prow = (size_t)(b * a.T + t) * a.G + hg;
     // all of the prefix's first parts are asked for at once, with their maxima and sums
-    constexpr int AHEAD = RG == 1 ? 16 : 8;
+    constexpr int AHEAD = RG == 1 && BLOCKS < 4 ? 16 : 8;
     float4 o[AHEAD];
     if (psplits > 0)
 #pragma unroll
@@ -400,13 +400,13 @@ k_attn_rows(RowsArgs a, int* status) {
 }
 
 // How a launch splits: row tiles, tile groups, CTAs of a cluster, clusters of a (sequence, kv head), ring stages.
-struct RowsPlan { int rg, dg, splits, clusters, stages, share; size_t smem; };
+struct RowsPlan { int rg, dg, per_sm, splits, clusters, stages, share; size_t smem; };
 
 typedef void (*rows_kernel)(RowsArgs, int*);
 rows_kernel rows_form(const RowsPlan& p) {
   if (p.rg == 4) return k_attn_rows<4, 1, 1>;
   if (p.rg == 2) return k_attn_rows<2, 1, 2>;
-  return p.dg == 3 ? k_attn_rows<1, 3, 1> : k_attn_rows<1, 1, 3>;
+  return p.dg == 3 ? k_attn_rows<1, 3, 1> : p.per_sm == 4 ? k_attn_rows<1, 1, 4> : k_attn_rows<1, 1, 3>;
 }
 
 size_t rows_smem(const RowsPlan& p, int rows) {
@@ -415,7 +415,7 @@ size_t rows_smem(const RowsPlan& p, int rows) {
 
 // Fills in the ring and the sizes for `each` pages a split.
 void rows_sizes(RowsPlan& p, int rows, long long each) {
-  p.stages = p.rg == 4 ? 6 : 3;
+  p.stages = p.rg == 4 ? 6 : p.per_sm == 4 ? 1 : p.per_sm == 3 ? 2 : 3;
   const int need = (4 * p.dg * rows * (ROW_LD + 2) * 4 + ROW_STAGE - 1) / ROW_STAGE;       // the warps' states lie over the ring
   if (each < p.stages) p.stages = each < 1 ? 1 : (int)each;
   if (p.dg == 3) p.stages = 3;                    // a stage always belongs to the same group, which tracks its parity
@@ -478,6 +478,10 @@ RowsPlan rows_plan(int vh, int rows, long long pages, bool join) {
     if (n > pages / p.splits) n = pages / p.splits;
     p.clusters = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
   }
+  // More unsplit pairs than two for an SM: a ring of two stages leaves room for a third, one stage for a fourth, where
+  // that saves the second wave. 32 / 8 heads, two to an SM / so, us: 50 sequences under a window of 512 28.6 / 22.4, 48
+  // under 300 20.4 / 15.7; 64 under 512 31.5 / 30.3, 64 x 333 keys 21.7 / 20.0, 64 under 1024 49.3 / 49.4.
+  if (p.rg == 1 && p.dg == 1 && p.splits == 1 && vh > 2 * 148 && vh <= 4 * 148) p.per_sm = vh <= 3 * 148 ? 3 : 4;
   rows_sizes(p, rows, (pages + (long long)p.splits * p.clusters - 1) / ((long long)p.splits * p.clusters));
   return p;
 }
@@ -487,9 +491,9 @@ int rows_launch(const RowsPlan& p, RowsArgs& a, int vh, const char* who, cudaStr
   if (!status) { q_set_error("%s: could not locate the device status word", who); return Q_ERR_CUDA; }
   a.share = p.share;
   a.stages = p.stages;
-  static size_t done[4][64] = {{0}};
+  static size_t done[5][64] = {{0}};
   const rows_kernel k = rows_form(p);
-  Q_CHECK_CUDA(q_ensure_smem(k, p.smem, done[p.rg == 4 ? 3 : p.rg == 2 ? 2 : p.dg == 3 ? 1 : 0]));
+  Q_CHECK_CUDA(q_ensure_smem(k, p.smem, done[p.rg == 4 ? 3 : p.rg == 2 ? 2 : p.dg == 3 ? 1 : p.per_sm == 4 ? 4 : 0]));
   Q_CHECK_CUDA(q_launch_cluster(k, dim3(p.splits * p.clusters, vh), dim3((4 * p.rg * p.dg + 1) * 32), p.smem, stream,
                                 (unsigned)p.splits, a, status));
   return Q_OK;
