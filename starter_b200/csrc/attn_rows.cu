@@ -424,6 +424,12 @@ void rows_sizes(RowsPlan& p, int rows, long long each) {
   p.smem = rows_smem(p, rows);
 }
 
+// Lets a form have the shared memory of a plan (only ever more: the limit is the kernel's, not the launch's).
+cudaError_t rows_room(const RowsPlan& p) {
+  static size_t done[5][64] = {{0}};
+  return q_ensure_smem(rows_form(p), p.smem, done[p.rg == 4 ? 3 : p.rg == 2 ? 2 : p.dg == 3 ? 1 : p.per_sm == 4 ? 4 : 0]);
+}
+
 // Clusters of a form that the current device holds at once (a cluster stays inside one GPC, so this is less than
 // the SMs would allow), asked once per device.
 int rows_resident(const RowsPlan& p) {
@@ -437,7 +443,7 @@ int rows_resident(const RowsPlan& p) {
     rows_sizes(full, 8 * p.rg, 1 << 20);
     const rows_kernel k = rows_form(full);
     int got = 0;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)full.smem);
+    cudaError_t e = rows_room(full);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.splits);
     cfg.blockDim = dim3((4 * p.rg * p.dg + 1) * 32);
@@ -491,9 +497,8 @@ int rows_launch(const RowsPlan& p, RowsArgs& a, int vh, const char* who, cudaStr
   if (!status) { q_set_error("%s: could not locate the device status word", who); return Q_ERR_CUDA; }
   a.share = p.share;
   a.stages = p.stages;
-  static size_t done[5][64] = {{0}};
   const rows_kernel k = rows_form(p);
-  Q_CHECK_CUDA(q_ensure_smem(k, p.smem, done[p.rg == 4 ? 3 : p.rg == 2 ? 2 : p.dg == 3 ? 1 : p.per_sm == 4 ? 4 : 0]));
+  Q_CHECK_CUDA(rows_room(p));
   Q_CHECK_CUDA(q_launch_cluster(k, dim3(p.splits * p.clusters, vh), dim3((4 * p.rg * p.dg + 1) * 32), p.smem, stream,
                                 (unsigned)p.splits, a, status));
   return Q_OK;

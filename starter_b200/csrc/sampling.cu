@@ -996,6 +996,13 @@ k_sample(const SampleArgs a) {
   }
 }
 
+// Lets a kernel have that much shared memory (only ever more: the limit is the kernel's, not the launch's).
+template <typename T, int THREADS>
+cudaError_t sample_room(size_t bytes) {
+  static size_t done[64] = {0};
+  return q_ensure_smem(k_sample<T, THREADS>, bytes, done);
+}
+
 // Clusters of a size that the current device holds at once, a CTA to an SM (a cluster stays inside one GPC, so this is
 // less than the SMs would allow), asked once per device.
 int sample_resident(int ctas) {
@@ -1014,7 +1021,7 @@ int sample_resident(int ctas) {
     at[0].val.clusterDim.x = ctas; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = 1;
     int got = 0;
-    cudaError_t e = cudaFuncSetAttribute(k_sample<bf16, SM_THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    cudaError_t e = sample_room<bf16, SM_THREADS>(bytes);
     if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&got, k_sample<bf16, SM_THREADS>, &cfg);
     if (e != cudaSuccess) { cudaGetLastError(); got = 132 / ctas; }
     n = got > 0 ? got : -1;
@@ -1030,8 +1037,7 @@ int sample_launch(SampleArgs a, int rows, int ctas, cudaStream_t stream) {
   const size_t slice = (size_t)a.seg * (THREADS / 32) * sizeof(T);
   a.resident = slice <= SM_SLICE;              // (otherwise every pass reads the row again, from L2)
   const size_t bytes = (sizeof(SampleShared) + 15) / 16 * 16 + (a.resident ? slice : 0);
-  static size_t done[64] = {0};
-  Q_CHECK_CUDA(q_ensure_smem(k_sample<T, THREADS>, bytes, done));
+  Q_CHECK_CUDA((sample_room<T, THREADS>(bytes)));
   Q_CHECK_CUDA(q_launch_cluster(k_sample<T, THREADS>, dim3((unsigned)rows * ctas), dim3(THREADS), bytes, stream, (unsigned)ctas, a));
   return Q_OK;
 }

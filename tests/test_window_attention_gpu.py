@@ -144,3 +144,19 @@ def test_captured_and_on_another_stream(ops):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, got)
+
+
+def test_shapes_of_every_split_count_one_after_the_other(ops):
+    """The first call of a split count asks how many clusters are resident; that must not take shared memory from a
+    shape that has run before."""
+    shapes = [(1, 32, 8, 1000), (2, 16, 8, 700), (5, 32, 8, 500), (20, 32, 8, 300), (40, 32, 8, 200), (70, 32, 8, 100), (3, 32, 8, 5000)]
+    made = []
+    for again in range(2):
+        for B, nq, nkv, capacity in shapes:
+            attn = ops.WindowAttention(B, nq, nkv, capacity, "cuda", 400, 4)
+            cache = ops.PagedKV(B, nkv, capacity, "cuda")
+            q = torch.ones((B, nq, 128), dtype=torch.bfloat16, device="cuda")
+            cache.v.fill_(2.0)
+            made.append(attn.run(q, cache, torch.full((1,), capacity - 1, dtype=torch.int32, device="cuda"), SCALE))
+    torch.cuda.synchronize()
+    assert all(bool((x == 2.0).all()) for x in made)
