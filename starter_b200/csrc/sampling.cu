@@ -320,7 +320,7 @@ k_sample(const SampleArgs a) {
   if (!(temperature > 0.f) || top_p <= 0.f) top_k = 1;               // the largest alone
   if (!(temperature > 0.f)) temperature = 1.f;
   if (top_k <= 0 || top_k >= a.vocab) top_k = 0;
-  const bool by_min = min_p > 0.f;
+  const bool by_min = min_p > 0.f && temperature < INFINITY;         // (NaN: off; at an infinite temperature all weigh the same)
   min_p = fminf(min_p, 1.f);
   Weigher weigh;
   weigh.rate = 16 * 1.4426950408889634074 / (double)temperature;

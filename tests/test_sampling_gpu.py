@@ -141,6 +141,33 @@ def test_extreme_logits(ops, scale, settings):
     check(ops, x, u, temperature=scale, **settings)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=40), dict(top_k=2000), dict(top_p=0.9), dict(min_p=0.01)], ids=str)
+def test_masks_of_the_lowest_value(ops, dtype, settings):
+    """Banned by the type's lowest number instead of -inf: of no weight, though they count as logits."""
+    x, u = rows_of(5, 7001, dtype, 61)
+    x[:, ::3] = torch.finfo(dtype).min
+    x[4, 10:] = torch.finfo(dtype).min
+    check(ops, x, u, **settings)
+
+
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=40), dict(top_p=0.5), dict(min_p=0.5), dict(min_p=1.0)], ids=str)
+def test_infinite_temperature(ops, settings):
+    """Every logit that is not -inf weighs the same."""
+    x, _ = rows_of(3, 3000, torch.float32, 62)
+    x[1, :100] = -math.inf
+    u = torch.tensor([0.1234567, 0.5, 0.987654])
+    tokens, logprobs = ops.sample_tokens(x.cuda(), u.cuda(), temperature=math.inf, **settings)
+    for r in range(3):
+        order = torch.sort(x[r], descending=True, stable=True)[1]
+        order = order[x[r][order] > -math.inf]
+        n = settings.get("top_k", len(order))
+        n = math.ceil(n * settings.get("top_p", 1.0))
+        kept = order[:n].sort()[0]
+        assert tokens[r].item() == kept[int(u[r].double() * n)].item()
+        assert abs(logprobs[r].item() + math.log(n)) <= 1e-6
+
+
 def test_strides(ops):
     x, u = rows_of(6, 5001, torch.bfloat16, 30)
     wide = torch.full((6, 5555), math.nan, dtype=torch.bfloat16, device="cuda")
