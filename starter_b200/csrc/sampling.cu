@@ -8,14 +8,15 @@
 //
 // All three cuts are thresholds on x plus a count of equal values taken by index, so no row is sorted, only a short
 // list. A cluster of CTAs holds a row in shared memory and reads it from memory once. After its maximum:
-//  - top-k (with or without the others): the j-th largest of the maxima of pairs of threads is at most the
-//    j-th largest value, so that the values from it on hold the top j, and are hardly more. They go on a list in
+//  - top-k (with or without the others): the j-th largest of the maxima of 256 groups of threads is at most
+//    the j-th largest value, so that the values from it on hold the top j, and are hardly more. They go on a list in
 //    one CTA, which sorts it, cuts it by prefix sums, sorts the rest by index and finds the token by prefix sums
 //    again. The same with min-p alone: its threshold is known.
 //  - top-p alone: a histogram of counts over 4096 equal parts of the value range gives the sums to a fraction of
-//    a percent (and for a top-k of thousands the part of its cut), and with that the few parts in which the cut must lie. One pass over the row then takes the exact
-//    sum of all w and, by stretch (a warp's run of indexes), of those above these parts, whose values go on the
-//    list; there the cut is found, then the stretch of the token, and its warp finds the token in it.
+//    a percent (and for a top-k of thousands the part of its cut), and with that the few parts in which the cut
+//    must lie. One pass over the row then takes the exact sum of all w and, by stretch (a warp's run of indexes),
+//    of those above these parts, whose own values go on the list; there the cut is found, then the stretch of the
+//    token, and its warp finds the token in it.
 //  - no filter: the stretches' sums, and one stretch again.
 //  - whatever does not fit the list (thousands of equal values, top-p behind a top-k of thousands): histograms of counts and
 //    exact sums, level by level, down to a single value.
@@ -38,7 +39,6 @@ constexpr int SM_CTAS = 8;                     // CTAs of a cluster at most
 constexpr int SM_FRACTION = 44;                // bits of a weight
 constexpr int SM_MAX_VOCAB = 1 << 19;          // (sums of so many stay below 2^63)
 constexpr int SM_MOST = 1 << 17;               // values of a CTA at most (their 15-bit pieces add up in 32 bits)
-constexpr size_t SM_SLICE = 180 * 1024;        // most bytes of a row's part that a CTA keeps
 
 typedef unsigned long long u64;
 
@@ -82,6 +82,9 @@ struct SampleShared {
     struct { unsigned count[SM_THREADS], mass[3][SM_THREADS], all_count[SM_THREADS]; u64 all_mass[SM_THREADS]; } level;
   };
 };
+
+constexpr size_t SM_SMEM_MAX = 227 * 1024;     // of a CTA: the above and the part of the row that it keeps, if that fits
+constexpr size_t SM_FIXED = (sizeof(SampleShared) + 15) / 16 * 16;
 
 __device__ __forceinline__ uint32_t shared_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ uint32_t at_rank(const void* p, int rank) {
@@ -275,7 +278,7 @@ k_sample(const SampleArgs a) {
   constexpr int VEC = Vec<T>::N;
   extern __shared__ __align__(16) unsigned char smem[];
   SampleShared& sh = *reinterpret_cast<SampleShared*>(smem);
-  uint4* slice = reinterpret_cast<uint4*>(smem + (sizeof(SampleShared) + 15) / 16 * 16);
+  uint4* slice = reinterpret_cast<uint4*>(smem + SM_FIXED);
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t rank, ctas;
@@ -996,11 +999,12 @@ k_sample(const SampleArgs a) {
   }
 }
 
-// Lets a kernel have that much shared memory (only ever more: the limit is the kernel's, not the launch's).
+// (The limit is the kernel's, not the launch's: one that never moves cannot be lowered by another shape's launch, or by
+// one of another thread.)
 template <typename T, int THREADS>
-cudaError_t sample_room(size_t bytes) {
+cudaError_t sample_room() {
   static size_t done[64] = {0};
-  return q_ensure_smem(k_sample<T, THREADS>, bytes, done);
+  return q_ensure_smem(k_sample<T, THREADS>, SM_SMEM_MAX, done);
 }
 
 // Clusters of a size that the current device holds at once, a CTA to an SM (a cluster stays inside one GPC, so this is
@@ -1011,17 +1015,16 @@ int sample_resident(int ctas) {
   if (dev < 0) return 132 / ctas;
   int& n = cached[dev][ctas];
   if (n == 0) {
-    const size_t bytes = sizeof(SampleShared) + 16 + SM_SLICE;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(SM_THREADS);
-    cfg.dynamicSmemBytes = bytes;
+    cfg.dynamicSmemBytes = SM_SMEM_MAX;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = ctas; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = 1;
     int got = 0;
-    cudaError_t e = sample_room<bf16, SM_THREADS>(bytes);
+    cudaError_t e = sample_room<bf16, SM_THREADS>();
     if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&got, k_sample<bf16, SM_THREADS>, &cfg);
     if (e != cudaSuccess) { cudaGetLastError(); got = 132 / ctas; }
     n = got > 0 ? got : -1;
@@ -1035,9 +1038,9 @@ int sample_launch(SampleArgs a, int rows, int ctas, cudaStream_t stream) {
   const long long stretches = (long long)ctas * (THREADS / 32);
   a.seg = (int)((a.vocab + VEC - 1 + stretches * VEC - 1) / (stretches * VEC)) * VEC;
   const size_t slice = (size_t)a.seg * (THREADS / 32) * sizeof(T);
-  a.resident = slice <= SM_SLICE;              // (otherwise every pass reads the row again, from L2)
-  const size_t bytes = (sizeof(SampleShared) + 15) / 16 * 16 + (a.resident ? slice : 0);
-  Q_CHECK_CUDA((sample_room<T, THREADS>(bytes)));
+  a.resident = SM_FIXED + slice <= SM_SMEM_MAX;      // (otherwise every pass reads the row again, from L2)
+  const size_t bytes = SM_FIXED + (a.resident ? slice : 0);
+  Q_CHECK_CUDA((sample_room<T, THREADS>()));
   Q_CHECK_CUDA(q_launch_cluster(k_sample<T, THREADS>, dim3((unsigned)rows * ctas), dim3(THREADS), bytes, stream, (unsigned)ctas, a));
   return Q_OK;
 }
