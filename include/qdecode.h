@@ -361,7 +361,8 @@ int q_attention_prefill(const void* d_q, const q_kv_layout_t* kv, const int32_t*
  *
  * q_attention_window: q_attention under a sliding window with sinks. Row (b, t, head) sits at
  * p = pos + t and attends to keys j <= p with j > p - window or j < sinks. d_q [batch*T][n_q][128],
- * T * n_q / n_kv <= 32; one launch, no scratch. A row that sees no key (a negative position) gives zeros. */
+ * T * n_q / n_kv <= 32, d_out 8-byte aligned; one launch, no scratch. A row that sees no key (a negative position)
+ * gives zeros. */
 int q_attention_window(const void* d_q, const q_kv_layout_t* kv, const int32_t* d_pos, int pos_per_seq,
                        void* d_out, int batch, int T, int n_q_heads, int window, int sinks, float scale,
                        void* stream);
@@ -375,9 +376,9 @@ int q_attention_window_prefill(const void* d_q, const q_kv_layout_t* kv, const i
 /* Attention of a batch that shares a prefix: row (b, t, head) attends to keys [0, *d_prefix_len) of the one
  * sequence in `prefix`, read once for the whole batch, and to keys [0, pos + t] of sequence b in `kv` (which may lie
  * in the same pools). Two launches: the prefix in key splits that leave partial results in d_scratch
- * (q_attention_shared_scratch_bytes(), 16-byte aligned; one call at a time may use it), then the sequences' own keys, joined
- * with them. T * n_q / n_kv <= 32. A prefix length beyond the prefix's pages is cut to them; a row
- * that sees no key gives zeros. 0 bytes: sizes that q_attention_shared refuses. */
+ * (q_attention_shared_scratch_bytes(), 16-byte aligned; one call at a time may use it), then the sequences' own
+ * keys, joined with them. T * n_q / n_kv <= 32, d_out 8-byte aligned. A prefix length beyond the prefix's pages is cut
+ * to them; a row that sees no key gives zeros. 0 bytes: sizes that q_attention_shared refuses. */
 int64_t q_attention_shared_scratch_bytes(int batch, int T, int n_q_heads, int n_kv_heads, int prefix_pages);
 int q_attention_shared(const void* d_q, const q_kv_layout_t* prefix, const int32_t* d_prefix_len,
                        const q_kv_layout_t* kv, const int32_t* d_pos, int pos_per_seq, void* d_scratch,
@@ -415,8 +416,8 @@ int q_logits_argmax(const float* d_branch, const q_gemm_plan_t* plan,
 
 /* ---- a token by chance ------------------------------------------------------
  * (No reference counterpart.) From bf16 (fp32 = 0) or fp32 logits [rows][vocab], rows row_stride values apart (0: every
- * row draws from the same logits): of every row the token that the random number d_uniform[row] in [0, 1) stands for, and the logarithm of its
- * probability in the set it was drawn from. With w_i = exp((x_i - max x) / temperature):
+ * row draws from the same logits): of every row the token that the random number d_uniform[row] in [0, 1) stands for,
+ * and the logarithm of its probability in the set it was drawn from. With w_i = exp((x_i - max x) / temperature):
  *   top_k:  the top_k largest logits, of equal ones those of the lowest index (0, negative, vocab and more: all);
  *   min_p:  of those the ones with w_i >= min_p, that is, of at least min_p times the largest probability (0: all);
  *   top_p:  of those, in descending order (equal ones by index), the shortest run with a sum of w of at least
@@ -668,7 +669,8 @@ int q_verify_step(q_engine* e, void* stream);
 
 /* Reads the library's device status words of the current device (synchronises the device;
  * not capturable). A non-zero word means a bounded wait inside a kernel ran out and the
- * results since then are not to be trusted: out[0] attention (1 producer, 2 consumer),
+ * results since then are not to be trusted: out[0] attention (1 producer, 2 consumer; on tensor memory
+ * 7 producer, 8 MMA issuer, 9 softmax),
  * out[1] stream-K GEMM ring (1), out[2] tcgen05 GEMM (1 producer, 2 MMA issuer, 3 epilogue,
  * 4 drain; prompt 5-8, whole projections 10-13 in the same order), out[3] tensor parallel over peer memory (1 = a peer's arrival word never came).
  * The words are sticky; q_clear_status zeroes them (synchronises too). */

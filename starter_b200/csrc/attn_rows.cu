@@ -18,7 +18,7 @@
 // as in the decode attention, so that few rows leave no accumulator empty. Four warps share a tile of 64 keys, 16
 // keys each; RG such groups take a row tile each, DG of them a key tile each. (With the row tiles in one warp's
 // registers, four at most, a tile of 64 keys and 32 rows took 2.9 us: one warp a scheduler hides none of the MMAs'
-// latency. As here 0.9.) Cast boundaries as there: fp32 scores and statistics, P rounded to bf16 for
+// latency. As here 1.9.) Cast boundaries as there: fp32 scores and statistics, P rounded to bf16 for
 // P V (the tensor cores' operand type), fp32 sums, one rounding of the result.
 //
 // Rows of a page that no query row sees may hold anything: their scores are replaced, their values cleared.
@@ -424,10 +424,12 @@ void rows_sizes(RowsPlan& p, int rows, long long each) {
   p.smem = rows_smem(p, rows);
 }
 
-// Lets a form have the shared memory of a plan (only ever more: the limit is the kernel's, not the launch's).
+// Lets a form have any plan's shared memory: the limit is the kernel's, not the launch's, and one that never moves
+// cannot be lowered by another shape's launch, or by one of another thread.
+constexpr size_t ROW_SMEM_MAX = 227 * 1024;
 cudaError_t rows_room(const RowsPlan& p) {
   static size_t done[5][64] = {{0}};
-  return q_ensure_smem(rows_form(p), p.smem, done[p.rg == 4 ? 3 : p.rg == 2 ? 2 : p.dg == 3 ? 1 : p.per_sm == 4 ? 4 : 0]);
+  return q_ensure_smem(rows_form(p), ROW_SMEM_MAX, done[p.rg == 4 ? 3 : p.rg == 2 ? 2 : p.dg == 3 ? 1 : p.per_sm == 4 ? 4 : 0]);
 }
 
 // Clusters of a form that the current device holds at once (a cluster stays inside one GPC, so this is less than

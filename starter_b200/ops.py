@@ -483,7 +483,7 @@ class SharedPrefixAttention:
             raise ValueError("unsupported shared-prefix attention metadata")
         self.batch, self.hq, self.hk, self.T = batch, query_heads, kv_heads, tokens_per_seq
         self.prefix_capacity, self.capacity = prefix_capacity, capacity
-        self._planned = self._scratch = 0          # prefix pages that the scratch size is for
+        self._planned = (0, 0)                     # prefix pages, and the scratch bytes that they take
 
     def run(self, query, prefix: PagedKV, prefix_length, cache: PagedKV, position, scale) -> torch.Tensor:
         """query [batch*T, Hq, 128] -> [batch*T, Hq*128]."""
@@ -497,12 +497,13 @@ class SharedPrefixAttention:
                 or prefix.device != device):
             raise ValueError("prefix_length must be an int32 tensor of shape [1], it and the prefix on the query's device")
         each = _positions(position, self.batch, device)
-        if prefix.pages_per_seq != self._planned:
-            self._scratch = lib.q_attention_shared_scratch_bytes(self.batch, self.T, self.hq, self.hk,
-                                                                 prefix.pages_per_seq)
-            self._planned = prefix.pages_per_seq
+        planned = self._planned
+        if prefix.pages_per_seq != planned[0]:
+            planned = (prefix.pages_per_seq, lib.q_attention_shared_scratch_bytes(
+                self.batch, self.T, self.hq, self.hk, prefix.pages_per_seq))
+            self._planned = planned
         out = torch.empty((self.batch * self.T, self.hq * HEAD_DIM), dtype=torch.bfloat16, device=device)
-        scratch = torch.empty(self._scratch or 16, dtype=torch.uint8, device=device)
+        scratch = torch.empty(planned[1] or 16, dtype=torch.uint8, device=device)
         _call(device, lib.q_attention_shared, query.data_ptr(), C.byref(prefix.layout), prefix_length.data_ptr(),
               C.byref(cache.layout), position.data_ptr(), each, scratch.data_ptr(), out.data_ptr(), self.batch, self.T,
               self.hq, scale)
