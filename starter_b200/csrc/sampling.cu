@@ -454,9 +454,9 @@ k_sample(const SampleArgs a) {
       unsigned b;
       asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(b) : "r"(at_rank(&sh.listed[which], 0)), "r"(found) : "memory");
       sh.base = b;
-      sh.found = 0;
     }
     __syncthreads();
+    if (tid == 0) sh.found = 0;                // (every thread has read it)
     if (tid < (int)min(found, (unsigned)THREADS) && sh.base + tid < THREADS) put64(&sh.list[sh.base + tid], 0, sh.spare[tid]);
     cluster_sync();
   };
