@@ -39,8 +39,9 @@ constexpr int SM_PER = 128;
 constexpr int SM_GROUPS = 256;                 // groups of threads whose maxima bound the top-k cut
 constexpr int SM_CTAS = 8;                     // CTAs of a cluster at most
 constexpr int SM_FRACTION = 44;                // bits of a weight
+constexpr int SM_MAX_ROWS = 1 << 24;
 constexpr int SM_MAX_VOCAB = 1 << 19;          // (sums of so many stay below 2^63)
-constexpr int SM_MOST = 1 << 17;               // values of a CTA at most (their 15-bit pieces add up in 32 bits)
+constexpr int SM_MOST = 1 << 17;               // values that a CTA gets at most (their 15-bit pieces add up in 32 bits)
 
 typedef unsigned long long u64;
 
@@ -1043,11 +1044,41 @@ int sample_resident(int ctas) {
   return n;
 }
 
+// Values of a warp's stretch: whole vectors, and the row may begin anywhere in its first one.
+template <typename T>
+int sample_seg(int vocab, int ctas, int threads) {
+  constexpr int VEC = Vec<T>::N;
+  const int vectors = ctas * (threads / 32) * VEC;
+  return (vocab + VEC - 1 + vectors - 1) / vectors * VEC;
+}
+
+// How a row is dealt out; most values that a CTA gets.
+struct SamplePlan { int ctas, threads, seg; };
+template <typename T>
+int sample_most(int vocab, int ctas, int threads) {
+  const int room = sample_seg<T>(vocab, ctas, threads) * (threads / 32);
+  return room < vocab ? room : vocab;
+}
+
+template <typename T>
+SamplePlan sample_plan(int rows, int vocab) {
+  // CTAs of a row: as many as leave all rows' clusters resident, while a CTA has a few thousand values. Not more where
+  // a CTA's part then does not fit its shared memory: 64 rows of 151936 in 32 bits with 4 CTAs in two waves / 2
+  // CTAs that read the row from L2 in each pass, us: top-k 33 / 23, top-p 71 / 62.
+  SamplePlan p;
+  p.ctas = 1;
+  while (p.ctas < SM_CTAS && vocab / (p.ctas * 2) >= 3000 && rows <= sample_resident(p.ctas * 2)) p.ctas *= 2;
+  // (stretches are rounded up to whole vectors: a CTA may get more than its share of the row)
+  while (sample_most<T>(vocab, p.ctas, SM_THREADS) > SM_MOST) p.ctas *= 2;
+  // Fewer threads meet faster, more hide the latency of the 64-bit arithmetic. 512 / 1024 threads, us: 1 row of 151936
+  // (19000 a CTA) top-p 22.7 / 25.1, 7 of 32003 top-k 10.7 / 11.4; 32 of 151936 (38000 a CTA) top-p 35.5 / 34.1.
+  p.threads = vocab / p.ctas < 24000 ? 512 : SM_THREADS;
+  p.seg = sample_seg<T>(vocab, p.ctas, p.threads);
+  return p;
+}
+
 template <typename T, int THREADS>
 int sample_launch(SampleArgs a, int rows, int ctas, cudaStream_t stream) {
-  constexpr int VEC = Vec<T>::N;
-  const long long stretches = (long long)ctas * (THREADS / 32);
-  a.seg = (int)((a.vocab + VEC - 1 + stretches * VEC - 1) / (stretches * VEC)) * VEC;
   const size_t slice = (size_t)a.seg * (THREADS / 32) * sizeof(T);
   a.resident = SM_FIXED + slice <= SM_SMEM_MAX;      // (otherwise every pass reads the row again, from L2)
   const size_t bytes = SM_FIXED + (a.resident ? slice : 0);
@@ -1057,26 +1088,31 @@ int sample_launch(SampleArgs a, int rows, int ctas, cudaStream_t stream) {
 }
 
 template <typename T>
-int sample_go(const SampleArgs& a, int rows, cudaStream_t stream) {
-  // CTAs of a row: as many as leave all rows' clusters resident, while a CTA has a few thousand values. Not more where
-  // a CTA's part then does not fit its shared memory: 64 rows of 151936 in 32 bits with 4 CTAs in two waves / 2
-  // CTAs that read the row from L2 in each pass, us: top-k 33 / 23, top-p 71 / 62.
-  int ctas = 1;
-  while (ctas < SM_CTAS && a.vocab / (ctas * 2) >= 3000 && rows <= sample_resident(ctas * 2)) ctas *= 2;
-  while (a.vocab / ctas > SM_MOST) ctas *= 2;
-  // Fewer threads meet faster, more hide the latency of the 64-bit arithmetic. 512 / 1024 threads, us: 1 row of 151936
-  // (19000 a CTA) top-p 22.7 / 25.1, 7 of 32003 top-k 10.7 / 11.4; 32 of 151936 (38000 a CTA) top-p 35.5 / 34.1.
-  return a.vocab / ctas < 24000 ? sample_launch<T, 512>(a, rows, ctas, stream) : sample_launch<T, 1024>(a, rows, ctas, stream);
+int sample_go(SampleArgs a, int rows, cudaStream_t stream) {
+  const SamplePlan p = sample_plan<T>(rows, a.vocab);
+  a.seg = p.seg;
+  return p.threads == 512 ? sample_launch<T, 512>(a, rows, p.ctas, stream) : sample_launch<T, 1024>(a, rows, p.ctas, stream);
 }
 
 }  // namespace
+
+extern "C" int q_sample_tokens_plan(int fp32, int rows, int vocab, int* ctas, int* values) {
+  const char* who = "q_sample_tokens_plan";
+  Q_CHECK_ARG(ctas && values, "%s: null pointer", who);
+  Q_CHECK_ARG(rows >= 1 && rows <= SM_MAX_ROWS && vocab >= 1 && vocab <= SM_MAX_VOCAB,
+              "%s: %d rows of %d values (1 to 2^24 rows of up to %d)", who, rows, vocab, SM_MAX_VOCAB);
+  const SamplePlan p = fp32 ? sample_plan<float>(rows, vocab) : sample_plan<bf16>(rows, vocab);
+  *ctas = p.ctas;
+  *values = fp32 ? sample_most<float>(vocab, p.ctas, p.threads) : sample_most<bf16>(vocab, p.ctas, p.threads);
+  return Q_OK;
+}
 
 extern "C" int q_sample_tokens(const void* d_logits, int fp32, int64_t row_stride, const float* d_uniform,
                                const q_sampling_t* sampling, int64_t* d_tokens, float* d_logprobs, int rows, int vocab,
                                void* stream) {
   const char* who = "q_sample_tokens";
   Q_CHECK_ARG(d_logits && d_uniform && sampling && d_tokens && d_logprobs, "%s: null pointer", who);
-  Q_CHECK_ARG(rows >= 1 && rows <= (1 << 24) && vocab >= 1 && vocab <= SM_MAX_VOCAB,
+  Q_CHECK_ARG(rows >= 1 && rows <= SM_MAX_ROWS && vocab >= 1 && vocab <= SM_MAX_VOCAB,
               "%s: %d rows of %d values (1 to 2^24 rows of up to %d)", who, rows, vocab, SM_MAX_VOCAB);
   Q_CHECK_ARG(row_stride >= 0, "%s: negative row stride", who);
   Q_CHECK_ARG(sampling->d_temperature || sampling->temperature >= 0.f, "%s: temperature is negative or NaN", who);
