@@ -427,8 +427,8 @@ int q_logits_argmax(const float* d_branch, const q_gemm_plan_t* plan,
  * temperature 0: the largest logit, of equal ones the lowest index. Logits that are -inf or NaN are never drawn; a row
  * that has no others gives token -1 and -inf. If +inf occurs, only it is drawn. Every setting is one number or, where
  * its pointer is set, one per row in device memory (there a NaN or negative temperature means 0, a NaN
- * top_p or min_p that it is off). Weights and sums are exact to 2^-44 of the largest weight, and the
- * result does not depend on the order of execution. vocab up to 2^19. One launch, no scratch. */
+ * top_p or min_p that it is off). A weight is exact to 0.6 times 2^-44 of the largest one, a sum of n
+ * weights to n times that, and the result does not depend on the order of execution. vocab up to 2^19. One launch, no scratch. */
 typedef struct q_sampling_t {
   float temperature;
   int32_t top_k;
