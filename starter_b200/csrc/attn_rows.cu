@@ -33,6 +33,7 @@ namespace {
 constexpr int ROW_TILE = Q_PAGE_TOKENS * 256;      // bytes of a K or V page tile
 constexpr int ROW_STAGE = 2 * ROW_TILE;
 constexpr int ROW_LD = 136;                        // floats of a row of the warps' merge area (rows on other banks)
+constexpr int ROW_FAR = 0x7fffffff - 64;           // positions and windows count up to this, so that their sums fit
 constexpr int MAX_SPLITS = 8;                      // CTAs of a cluster (the portable size)
 
 struct RowsArgs {
@@ -61,8 +62,8 @@ __device__ __forceinline__ Seen seen_of(const RowsArgs& a, int b) {
   const int room = a.pages_per_seq * Q_PAGE_TOKENS;
   int p = __ldcg(a.pos + (size_t)b * a.pos_step);
   if (a.flat) p = max(0, p) - a.T;                               // row T-1 is then the newest key
-  // positions outside the pages see what there is: nothing outside the table is read
-  s.pos = a.flat ? min(p, room - a.T) : min(max(p, -a.T), room);
+  // a position behind the pages sees what its window still holds of them; nothing outside the table is read
+  s.pos = a.flat ? min(p, room - a.T) : min(max(p, -a.T), ROW_FAR);
   s.lim = min(max(s.pos + a.T, 0), room);
   s.low = a.flat ? 0 : min(max(0, s.pos - a.window + 1), s.lim);
   s.sink_pages = (min(a.sinks, s.lim) + Q_PAGE_TOKENS - 1) / Q_PAGE_TOKENS;
@@ -537,7 +538,7 @@ RowsArgs rows_args(const void* d_q, const q_kv_layout_t* kv, const int32_t* d_po
   a.nq = n_q_heads;
   a.T = T;
   a.G = n_q_heads / kv->n_kv_heads;
-  a.window = 1 << 30;
+  a.window = ROW_FAR;
   a.scale_log2 = scale * 1.4426950408889634f;
   return a;
 }
@@ -552,8 +553,8 @@ extern "C" int q_attention_window(const void* d_q, const q_kv_layout_t* kv, cons
   if (rc) return rc;
   Q_CHECK_ARG(window >= 1 && sinks >= 0, "%s: window %d / sinks %d", who, window, sinks);
   RowsArgs a = rows_args(d_q, kv, d_pos, pos_per_seq, d_out, T, n_q_heads, scale);
-  a.window = window < (1 << 30) ? window : 1 << 30;
-  a.sinks = sinks < (1 << 30) ? sinks : 1 << 30;
+  a.window = window < ROW_FAR ? window : ROW_FAR;
+  a.sinks = sinks < ROW_FAR ? sinks : ROW_FAR;
   // most pages a sequence's rows can see: those of window + T - 1 consecutive keys, and the sinks'
   const long long all = kv->pages_per_seq;
   long long pages = ((long long)a.window + T - 2) / Q_PAGE_TOKENS + 2 + ((long long)a.sinks + Q_PAGE_TOKENS - 1) / Q_PAGE_TOKENS;
