@@ -368,8 +368,9 @@ int q_attention_window(const void* d_q, const q_kv_layout_t* kv, const int32_t* 
                        void* d_out, int batch, int T, int n_q_heads, int window, int sinks, float scale,
                        void* stream);
 
-/* q_attention_prefill under the same window: row (b, t, head) of T prompt tokens, any T, up to 32 query heads per kv
- * head. Positions are not negative; d_out 4-byte aligned. */
+/* q_attention_prefill under the same window: row (b, t, head) of T prompt tokens, any T up to 2^30, up to 32 query heads
+ * per kv head. A negative position counts as 0, one behind the pages sees what its window still holds of them; positions and
+ * windows count up to 2^31 - 512 - T. d_out 4-byte aligned. */
 int q_attention_window_prefill(const void* d_q, const q_kv_layout_t* kv, const int32_t* d_pos, int pos_per_seq,
                                void* d_out, int batch, int T, int n_q_heads, int window, int sinks, float scale,
                                void* stream);

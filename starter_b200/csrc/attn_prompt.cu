@@ -66,6 +66,7 @@ struct AttnShape {
   int wide;          // the output is 32-byte aligned
   float scale_log2;
   int pos_step, window, sinks, room;     // WINDOW: positions per sequence, keys that the table's pages hold (PARTS: too)
+  int far;                               // WINDOW: positions count up to it, so that their sums with T fit
   AttnParts parts;                       // PARTS
 };
 
@@ -100,14 +101,15 @@ __device__ __forceinline__ Item item_of_form(const AttnShape& sh, int w, int pos
     it.b = bh / sh.nkv;
     it.kh = bh - it.b * sh.nkv;
     it.q0 = (sh.blocks - 1 - blk) * sh.tiles * sh.tokens;
-    // positions outside the pages read nothing outside the table
-    it.pos = min(max(__ldcg(pos_ptr + (size_t)it.b * sh.pos_step), 0), sh.room - 1);
+    it.pos = min(max(__ldcg(pos_ptr + (size_t)it.b * sh.pos_step), 0), sh.far);
     it.max_limit = min(it.pos + min(it.q0 + sh.tiles * sh.tokens, sh.T), sh.room);
-    it.low = min(max(0, it.pos + it.q0 - sh.window + 1), it.max_limit - 1);
+    it.low = max(0, it.pos + it.q0 - sh.window + 1);
     it.sink_tiles = (min(sh.sinks, it.max_limit) + AP_KEYS - 1) / AP_KEYS;
-    const int first = max(it.sink_tiles, it.low / AP_KEYS);
+    // Nothing outside the table is read. A window that lies behind the pages still walks their last tile, of which
+    // then no key is live and neither page is read: an item has one tile at least.
+    const int last = (it.max_limit - 1) / AP_KEYS, first = max(it.sink_tiles, min(it.low / AP_KEYS, last));
     it.skip = first - it.sink_tiles;
-    it.n = it.sink_tiles + max(0, (it.max_limit + AP_KEYS - 1) / AP_KEYS - first);
+    it.n = it.sink_tiles + max(0, last + 1 - first);
     it.split = 0;
   } else {
     // query blocks of a (split, kv head) next to one another: they share its keys in L2
@@ -650,7 +652,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
         free_keys = t_last < sh.T ? pos + t_first + 1 : 0;
       } else if constexpr (FORM == WINDOW) {
         limit = min(it.pos + t + 1, sh.room);
-        low = it.pos + t + 1 - sh.window;
+        low = max(0, it.pos + t + 1 - sh.window);
         free_keys = min(it.pos + it.q0 + i * sh.tokens + (warp & 3) * 32 / sh.G + 1, sh.room);
         free_from = it.pos + it.q0 + i * sh.tokens + ((warp & 3) * 32 + 31) / sh.G + 1 - sh.window;
       } else {
@@ -837,6 +839,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
         continue;
       }
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // NaN stays NaN
+      const bool none = FORM == WINDOW && l == 0.f;        // (O may never have been written)
       const int head = FORM == CAUSAL ? row & (sh.G - 1) : row - tok * sh.G;
       bf16* dst = out + (((size_t)it.b * sh.T + t) * sh.nq + it.kh * sh.G + head) * 128 + COLS * part;
 #pragma unroll 1
@@ -846,7 +849,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
         if (live_row) {
           uint32_t u[8];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) u[q] = pack_bf16(o[2 * q] * inv, o[2 * q + 1] * inv);
+          for (int q = 0; q < 8; ++q) u[q] = none ? 0u : pack_bf16(o[2 * q] * inv, o[2 * q + 1] * inv);
           if (sh.wide) {
             asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                          ::"l"(dst + 16 * k), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]),
@@ -963,8 +966,10 @@ extern "C" int q_attention_window_prefill(const void* d_q, const q_kv_layout_t* 
   Q_CHECK_ARG(window >= 1 && sinks >= 0, "%s: window %d / sinks %d", who, window, sinks);
   AttnShape sh = {};
   sh.pos_step = pos_per_seq ? 1 : 0;
-  sh.window = window < (1 << 30) ? window : 1 << 30;
-  sh.sinks = sinks < (1 << 30) ? sinks : 1 << 30;
+  Q_CHECK_ARG(T <= (1 << 30), "%s: %d tokens", who, T);
+  sh.far = 0x7fffffff - 512 - (T > 0 ? T : 0);             // (a block of tokens ends at most 255 behind T)
+  sh.window = window < 0x7fffffff - 512 ? window : 0x7fffffff - 512;
+  sh.sinks = sinks;
   return prompt_launch<WINDOW>(who, sh, d_q, kv, d_pos, d_out, batch, T, n_q_heads, scale, stream);
 }
 

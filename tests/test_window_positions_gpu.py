@@ -61,3 +61,23 @@ def test_a_few_rows(ops, nq, nkv, T, window, sinks):
     if window == FAR:                                        # (counted up to 2^31 - 65, positions as well)
         positions = positions[:11]
     check(ops, run, len(positions), nq, nkv, T, positions, window, sinks, 192)
+
+
+@pytest.mark.parametrize("nq,nkv,T", [(4, 1, 40), (32, 8, 1), (8, 2, 129), (28, 4, 200), (32, 8, 500)])
+@pytest.mark.parametrize("window,sinks", [(10, 0), (64, 0), (70, 5), (300, 0), (1, 200), (FAR, 0)])
+def test_prompts(ops, nq, nkv, T, window, sinks):
+    """One query tile for a block and (the last shape) two; blocks that begin before the pages' end and end behind it."""
+    def run(q, cache, position):
+        return ops.window_prompt_attention(q, cache, position, T, SCALE, window, sinks)
+    positions = [384 - T // 2, 320, 383, 384, 1000, 0, -5, 2 ** 20, 2 ** 30]
+    if window != FAR:                                        # (counted up to 2^31 - 512 - T, positions as well)
+        positions += [FAR]
+    check(ops, run, len(positions), nq, nkv, T, positions, window, sinks, 384, begins=0)
+
+
+def test_prompts_wholly_behind_the_pages(ops):
+    """No row sees anything, and the first item of a block has nothing to read."""
+    for T in (1, 40, 300):
+        def run(q, cache, position):
+            return ops.window_prompt_attention(q, cache, position, T, SCALE, 50, 0)
+        check(ops, run, 3, 8, 2, T, [192 + 50, 500, 2 ** 30], 50, 0, 192, begins=0)
