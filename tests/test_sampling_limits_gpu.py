@@ -1,4 +1,5 @@
 """The sampler where its sums decide at their limits. Tolerances as in test_sampling_gpu.py."""
+import math
 from decimal import Decimal, localcontext
 
 import pytest
@@ -67,3 +68,24 @@ def test_weights_are_exact_to_less_than_a_unit(ops):
             assert Decimal("0.7") < (w - Decimal(e) * (w + 1 + s)) * 2 ** 44 < Decimal("0.9")
     tokens, _ = ops.sample_tokens(x.cuda(), u.cuda())
     assert tokens.tolist() == [0] * len(u)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("temperature", [1e36, 2e37, 3e38, math.inf])
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=40), dict(top_k=700), dict(top_k=3000), dict(top_p=0.5), dict(min_p=0.2),
+                                      dict(top_k=2500, top_p=0.7)], ids=str)
+def test_logits_whose_differences_leave_32_bits(ops, dtype, temperature, settings):
+    """From the type's lowest number nearly to its largest, at temperatures at which all of that weighs."""
+    g = torch.Generator().manual_seed(44)
+    x = ((torch.rand((5, 6001), generator=g) * 2 - 1) * 3.3e38).to(dtype)
+    x[1, ::3] = torch.finfo(dtype).min
+    x[2, 5] = torch.finfo(dtype).max
+    x[3] = torch.where(torch.rand(6001, generator=g) < 0.5, -3.2e38, 3e38).to(dtype)
+    x[4, 77] = math.inf
+    u = torch.tensor([0.1234567, 0.4703, 0.987654, 0.7712, 0.3])
+    tokens, logprobs = ops.sample_tokens(x.cuda(), u.cuda(), temperature=temperature, **settings)
+    for r in range(4):
+        token, logprob, border = sample(x[r], u[r].item(), temperature=temperature, **settings)
+        assert border > 1e-7 and tokens[r].item() == token, (r, border)
+        assert abs(logprobs[r].item() - logprob) <= 2.0 ** -24 * abs(logprob) + 1e-7
+    assert tokens[4].item() == 77 and logprobs[4].item() == 0
