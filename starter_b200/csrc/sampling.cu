@@ -128,14 +128,12 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 // three coefficients, at most 4.5e-15 off to either side, 0.08 units.
 struct Weigher {
   double top, rate;                            // M, 16 log2(e) / temperature
-  float topf, alive;                           // M, and the smallest x that may have a weight
+  float topf, floor;                           // M, and the (x - M) / 2 from which on w rounds to 0
   const double* power;
   __device__ __forceinline__ void start(float most, float temperature) {
     top = (double)most;
     topf = most;
-    // exp(-32) < 2^-46. (The sum's rounding is a value's own, at most twice as far below M. Differences of values would
-    // leave 32 bits where temperatures of 1e37 and more make them matter.)
-    alive = most == INFINITY ? INFINITY : fmaxf(most - 32.f * temperature, -FLT_MAX);
+    floor = -16.f * temperature;               // exp(-32) < 2^-46
   }
   // of a finite M and -64 <= z (anything else gives some number; no branches: the chains of several values run side by
   // side)
@@ -159,7 +157,8 @@ struct Weigher {
   }
   __device__ __forceinline__ u64 operator()(float x) const {
     const u64 w = plain(x);
-    return x == topf ? 1ull << SM_FRACTION : x >= alive ? w : 0;             // (also of infinities)
+    // (also of infinities; a whole difference can leave 32 bits where temperatures of 1e37 and more make it matter)
+    return x == topf ? 1ull << SM_FRACTION : fmaf(0.5f, x, -0.5f * topf) > floor ? w : 0;
   }
 };
 
@@ -517,9 +516,9 @@ k_sample(const SampleArgs a) {
   }
 
   // ---- top-p or a large top-k alone (min-p first, where it let too many in)
-  if ((by_p ? top_k == 0 : top_k > 0) && top < INFINITY && temperature > 1e-36f) {      // (parts_per is finite)
-    // (differences beyond 32 bits fall into the last part, at an infinite temperature too)
-    const float parts_per = (float)SM_PER / fminf(temperature, FLT_MAX);
+  // (parts_per is finite, and values whose difference from the largest leaves 32 bits weigh nothing)
+  if ((by_p ? top_k == 0 : top_k > 0) && top < INFINITY && temperature > 1e-36f && temperature < 1e30f) {
+    const float parts_per = (float)SM_PER / temperature;
     auto part_of = [&](float v) { return v == top ? 0 : min(SM_PARTS - 1, (int)((top - v) * parts_per)); };
     for (int i = tid; i < SM_PARTS; i += THREADS) sh.parts.count[i] = 0;
     __syncthreads();
@@ -602,11 +601,10 @@ k_sample(const SampleArgs a) {
     };
     bool fits = values_in(part0, part1) <= THREADS;
     const float from_part = (float)part0;
-    // (up to and with this one: the last part has no end)
-    const float to_part = !fits ? -1.f : part1 == SM_PARTS - 1 ? INFINITY : nextafterf((float)(part1 + 1), 0.f);
-    // The smallest value that may have a weight. (With it weights need no checks of their ends: 32 x 151936 bf16, top-p,
-    // with them / so, 40.2 / 38.2 us.)
-    const float alive_from = fmaxf(weigh.alive, least_f);
+    const float to_part = !fits ? from_part : part1 == SM_PARTS - 1 ? INFINITY : (float)(part1 + 1);
+    // The smallest value that may have a weight: the sum's rounding is a value's own, at most twice as far below M. (With it
+    // weights need no checks of their ends: 32 x 151936 bf16, top-p, with them / so, 40.2 / 38.2 us.)
+    const float alive_from = fmaxf(fmaxf(top + 2.f * weigh.floor, -FLT_MAX), least_f);
     u64 sum = 0, above = 0;
     for (int o = lane * VEC; o < a.seg; o += STEP) {
       float v[VEC];
@@ -623,13 +621,13 @@ k_sample(const SampleArgs a) {
           const bool alive = v[j0 + j] >= alive_from, over = at < from_part;
           if (alive) sum += w[j];
           if (alive && over) above += w[j];
-          listed |= !over && at <= to_part;
+          listed |= !over && at < to_part;
         }
         if (listed) {
 #pragma unroll
           for (int j = 0; j < SIDE; ++j) {
             const float at = (top - v[j0 + j]) * parts_per;
-            if (let_in(v[j0 + j]) && at >= from_part && at <= to_part) push(v[j0 + j], begin + o + j0 + j);
+            if (let_in(v[j0 + j]) && at >= from_part && at < to_part) push(v[j0 + j], begin + o + j0 + j);
           }
         }
       }
