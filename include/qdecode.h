@@ -362,8 +362,8 @@ int q_attention_prefill(const void* d_q, const q_kv_layout_t* kv, const int32_t*
  * q_attention_window: q_attention under a sliding window with sinks. Row (b, t, head) sits at
  * p = pos + t and attends to keys j <= p with j > p - window or j < sinks. d_q [batch*T][n_q][128],
  * T * n_q / n_kv <= 32, d_out 8-byte aligned; one launch, no scratch. A row that sees no key (a negative position, or
- * one so far behind the pages that its window holds nothing of them) gives zeros. Positions and windows count up to
- * 2^31 - 65. */
+ * one so far behind the pages that its window holds nothing of them) gives zeros. Positions count up to 2^31 - 65, windows
+ * up to 2^31 - 33. */
 int q_attention_window(const void* d_q, const q_kv_layout_t* kv, const int32_t* d_pos, int pos_per_seq,
                        void* d_out, int batch, int T, int n_q_heads, int window, int sinks, float scale,
                        void* stream);

@@ -33,7 +33,8 @@ namespace {
 constexpr int ROW_TILE = Q_PAGE_TOKENS * 256;      // bytes of a K or V page tile
 constexpr int ROW_STAGE = 2 * ROW_TILE;
 constexpr int ROW_LD = 136;                        // floats of a row of the warps' merge area (rows on other banks)
-constexpr int ROW_FAR = 0x7fffffff - 64;           // positions and windows count up to this, so that their sums fit
+constexpr int ROW_FAR = 0x7fffffff - 64;           // positions count up to this, so that their sums with T fit
+constexpr int ROW_ALL = 0x7fffffff - 32;           // a window that holds every key of every such position
 constexpr int MAX_SPLITS = 8;                      // CTAs of a cluster (the portable size)
 
 struct RowsArgs {
@@ -538,7 +539,7 @@ RowsArgs rows_args(const void* d_q, const q_kv_layout_t* kv, const int32_t* d_po
   a.nq = n_q_heads;
   a.T = T;
   a.G = n_q_heads / kv->n_kv_heads;
-  a.window = ROW_FAR;
+  a.window = ROW_ALL;
   a.scale_log2 = scale * 1.4426950408889634f;
   return a;
 }
@@ -553,8 +554,8 @@ extern "C" int q_attention_window(const void* d_q, const q_kv_layout_t* kv, cons
   if (rc) return rc;
   Q_CHECK_ARG(window >= 1 && sinks >= 0, "%s: window %d / sinks %d", who, window, sinks);
   RowsArgs a = rows_args(d_q, kv, d_pos, pos_per_seq, d_out, T, n_q_heads, scale);
-  a.window = window < ROW_FAR ? window : ROW_FAR;
-  a.sinks = sinks < ROW_FAR ? sinks : ROW_FAR;
+  a.window = window < ROW_ALL ? window : ROW_ALL;
+  a.sinks = sinks;
   // most pages a sequence's rows can see: those of window + T - 1 consecutive keys, and the sinks'
   const long long all = kv->pages_per_seq;
   long long pages = ((long long)a.window + T - 2) / Q_PAGE_TOKENS + 2 + ((long long)a.sinks + Q_PAGE_TOKENS - 1) / Q_PAGE_TOKENS;

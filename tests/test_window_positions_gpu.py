@@ -81,3 +81,26 @@ def test_prompts_wholly_behind_the_pages(ops):
         def run(q, cache, position):
             return ops.window_prompt_attention(q, cache, position, T, SCALE, 50, 0)
         check(ops, run, 3, 8, 2, T, [192 + 50, 500, 2 ** 30], 50, 0, 192, begins=0)
+
+
+@pytest.mark.parametrize("batch", [2, 40])
+def test_own_keys_of_a_shared_prefix(ops, batch):
+    """A position behind the own pages sees all that they hold."""
+    g = torch.Generator().manual_seed(batch)
+    nkv, G, T = 2, 4, 4
+    prefix, cache = ops.PagedKV(1, nkv, 100, "cuda"), ops.PagedKV(batch, nkv, 64, "cuda")
+    k0, v0 = (torch.randn((1, nkv, 100, 128), generator=g).to(torch.bfloat16) for _ in range(2))
+    k, v = (torch.randn((batch, nkv, 64, 128), generator=g).to(torch.bfloat16) for _ in range(2))
+    prefix.scatter(k0.cuda(), v0.cuda(), 0)
+    cache.scatter(k.cuda(), v.cuda(), 0)
+    q = torch.randn((batch * T, nkv * G, 128), generator=g).to(torch.bfloat16)
+    attn = ops.SharedPrefixAttention(batch, nkv * G, nkv, 100, 64, "cuda", T)
+    positions = [FAR, 64] + [2 ** 20] * (batch - 2)
+    got = attn.run(q.cuda(), prefix, torch.tensor([100], dtype=torch.int32, device="cuda"), cache,
+                   torch.tensor(positions, dtype=torch.int32, device="cuda"), SCALE).cpu().view(batch, T, nkv * G, 128)
+    for b in {0, 1, batch - 1}:
+        for h in range(nkv):
+            keys, values = torch.cat([k0[0, h], k[b, h]]), torch.cat([v0[0, h], v[b, h]])
+            rows = q.view(batch, T, nkv * G, 128)[b, :, h * G:(h + 1) * G].reshape(T * G, 128)
+            want, bound = attend(rows, keys, values, torch.ones((T * G, 164), dtype=torch.bool), SCALE)
+            assert_close(got[b, :, h * G:(h + 1) * G].reshape(T * G, 128), want, bound)
