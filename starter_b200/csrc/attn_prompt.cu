@@ -20,10 +20,10 @@
 // Warp 16: producer lane. Warp 17: MMA issue; the whole warp walks the loop and one elected lane
 // issues, so that descriptors live in uniform registers: an MMA of 128 x 128 x 16 takes 64 cycles,
 // about what a single diverged lane needs to assemble its operands.
-// O is rescaled only when some row of the warp has a new maximum. (Moving the maximum only after
-// it had grown by 2^8 measured 367 against 390 us at 7000 tokens, but the largest probability of a
+// O is rescaled only when some row of the warp has a new maximum. (In the causal form. Moving the maximum
+// only after it had grown by 2^8 measured 367 against 390 us at 7000 tokens there, but the largest probability of a
 // row is then no longer exactly 1 in bf16: error against fp64 2.1e-3 instead of 1.77e-3 where scores
-// keep growing.) Cast boundaries as in attention.cu: fp32 scores and statistics, P rounded to bf16,
+// keep growing. The other two forms take that speed; what it costs them stands at the rescaling.) Cast boundaries as in attention.cu: fp32 scores and statistics, P rounded to bf16,
 // fp32 accumulation, one rounding of the result.
 //
 // Tiles are read through tensor maps whose boxes undo the 256-byte row pitch of a page: a box of
@@ -37,7 +37,7 @@
 // Three forms (FORM) walk other keys with the same pipeline: CAUSAL (the prompt), WINDOW (the prompt under a
 // sliding window with sinks: of the key tiles only those that hold a key some row of the item sees), PARTS (many
 // rows over one range of keys that all of them see, cut into key splits whose m, l and O are left in 32 bits).
-// In the last two any head count per kv head up to 128 is taken, k steps of 16 keys that nobody sees are left out
+// In the last two any head count per kv head up to 32 is taken, k steps of 16 keys that nobody sees are left out
 // of P V, and of a tile that nobody sees in one of its pages that page is not read.
 #include "tc.cuh"
 #include "attn_parts.cuh"
@@ -751,8 +751,11 @@ k_attn_prompt(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ 
         } else {
           // (the other forms let it grow by 2^8 first: over few tiles some row of a warp has a new maximum in nearly
           // each, and reading and writing O took a quarter of a step. P is then at most 256, as exact in bf16 as up to
-          // 1; only a row's largest is no longer exactly 1. A prompt of 7000 tokens under a window of 1024, at once / after
-          // 2^8, us: 174 / 163; of 5000 under 4096: 221 / 207.)
+          // 1; only a row's largest is no longer exactly 1. At once / after 2^8, us: a prompt of 7000 tokens under a window
+          // of 1024 176 / 165, under 4096 365 / 339, 3 x 701 50.5 / 48.0, 64 x 2 tokens over a prefix of 30001 82.8 / 77.9. Error
+          // against fp64, relative 2-norm, of unit normals 2.12e-3 / 2.20e-3 (windows), 2.26e-3 / 2.33e-3 (prefixes); where
+          // keys grow from 0.05 to 4 times that along the context 1.78e-3 / 2.19e-3 and 1.72e-3 / 2.09e-3, the largest error,
+          // of the largest result, 2.3e-3 / 4.7e-3 and 2.1e-3 / 3.8e-3. The result's own rounding is 1.66e-3 of that.)
           if (__any_sync(0xffffffffu, FORM == CAUSAL ? m_tile > m : (m_tile - m) * c > 8.f)) {
             // the products up to the tile before are complete: this tile's scores came after them (DEEP: after those
             // of the tile before that, so that the parity of the last ones names them)
@@ -914,6 +917,12 @@ int prompt_launch(const char* who, AttnShape& sh, const void* d_q, const q_kv_la
   // shorter chain. Up to two tiles per SM the one is faster. One tile / two, us: 1 x 592 tokens 15.5 / 18.8, 1 x 1024
   // 22.8 / 26.4, 1 x 1184 (296 tiles) 28.8 / 30.7, 3 x 250 10.2 / 12.8, 9 x 128 10.2 / 10.5, but 1 x 1200 32.4 / 31.8,
   // 3 x 400 (312) 19.4 / 17.0, 2 x 701 26.9 / 22.8. (With half of the warps idle, one tile took 17.1 at 592.)
+  // These are the causal form's; one tile of the other forms is DEEP. Windows, 32 / 8 heads, one / two, us: 1.7 row tiles per
+  // SM (1 x 1024) 19.5 / 22.7, 2.0 (1 x 1184 behind 2000, window 1024) 36.2 / 62.5, 2.4 (2 x 701 behind 1000, 512) 39.8 / 47.3,
+  // 3.6 (3 x 701) 51.6 / 48.0, 4.8 (4 x 701) 63.4 / 69.5, 7.1 (6 x 701) 101.9 / 91.3, 11.8 (1 x 7000, 1024) 182 / 165: up to
+  // two and from six on the rule holds; between them it goes by how full the last round of items is, which the rule does not
+  // look at. Prefixes, row tiles: 1 (32 x 16384) 25.8 / 32.8, 2 (64 x 16384) 34.0 / 37.8, 3 (96 x 16384) 45.6 / 54.1, 4 (64 x 2
+  // over 4096) 27.9 / 32.3 but over 30001 86.3 / 78.0, 8 (128 x 2 over 8192) 69.3 / 69.6.
   const int sms = q_sm_count();
   const long long row_tiles = (T + sh.tokens - 1) / sh.tokens;
   if (FORM == PARTS) sh.tiles = row_tiles == 1 ? 1 : 2;
