@@ -358,6 +358,7 @@ int q_attention_prefill(const void* d_q, const q_kv_layout_t* kv, const int32_t*
  * int32[batch]. Positions, tables, queries and keys may come from the launch right before; nothing
  * outside the block table's rows is read, whatever the position says, and no page that holds no visible key (the
  * table may say anything there). What pages hold in places nobody sees may be anything, NaN too.
+ * (An infinite or NaN value that one row sees may make NaN of other rows of the same sequence and kv head, as 0 * inf does.)
  * Scores, maxima and sums in 32 bits; probabilities are rounded to bf16 for the product with V, as in q_attention and
  * q_attention_prefill. The windowed prompt, and a shared prefix of more than 32 rows a kv head, take a row's maximum anew only
  * when it has grown by 2^8 (5 % faster), so that its largest probability is rounded too: relative error against 64 bits
