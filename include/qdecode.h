@@ -450,9 +450,10 @@ int q_sample_tokens(const void* d_logits, int fp32, int64_t row_stride, const fl
                     const q_sampling_t* sampling, int64_t* d_tokens, float* d_logprobs, int rows, int vocab,
                     void* stream);
 
-/* How q_sample_tokens deals out a row on the current device: the CTAs that share it, and the most values that one
- * of them gets (2^17 at most: sums of pieces of their weights are kept in 32 bits). */
-int q_sample_tokens_plan(int fp32, int rows, int vocab, int* ctas, int* values);
+/* How q_sample_tokens deals out a row on the current device (aligned: all rows begin on 16-byte boundaries): the CTAs
+ * that share it, and the most values that one of them gets (2^17 at most: sums of pieces of their weights are kept in
+ * 32 bits). */
+int q_sample_tokens_plan(int fp32, int rows, int vocab, int aligned, int* ctas, int* values);
 
 /* Final pick over tensor-parallel shards: val/idx are [shards][rows]; lowest
  * global index wins ties. Writes tokens and bumps *d_pos like above. */

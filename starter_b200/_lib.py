@@ -162,7 +162,7 @@ SIGNATURES = {
     "q_argmax_scratch_bytes": (C.c_int64, [_I, _I]),
     "q_logits_argmax": (_I, [_P, _PLAN, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P]),
     "q_sample_tokens": (_I, [_P, _I, C.c_int64, _P, C.POINTER(Sampling), _P, _P, _I, _I, _P]),
-    "q_sample_tokens_plan": (_I, [_I, _I, _I, C.POINTER(_I), C.POINTER(_I)]),
+    "q_sample_tokens_plan": (_I, [_I, _I, _I, _I, C.POINTER(_I), C.POINTER(_I)]),
     "q_argmax_merge": (_I, [_P, _P, _I, _I, _P, _P, _I, _P]),
     "q_create": (_I, [C.POINTER(Config), C.POINTER(_P)]),
     "q_bind_layer": (_I, [_P, _I, C.POINTER(LayerWeights)]),

@@ -1054,36 +1054,38 @@ int sample_resident(int ctas) {
   return n;
 }
 
-// Values of a warp's stretch: whole vectors, and the row may begin anywhere in its first one.
+// Values of a warp's stretch: whole vectors; a row that is not aligned may begin anywhere in its first one.
 template <typename T>
-int sample_seg(int vocab, int ctas, int threads) {
+int sample_seg(int vocab, bool aligned, int ctas, int threads) {
   constexpr int VEC = Vec<T>::N;
   const int vectors = ctas * (threads / 32) * VEC;
-  return (vocab + VEC - 1 + vectors - 1) / vectors * VEC;
+  return (vocab + (aligned ? 0 : VEC - 1) + vectors - 1) / vectors * VEC;
 }
 
 // How a row is dealt out; most values that a CTA gets.
 struct SamplePlan { int ctas, threads, seg; };
 template <typename T>
-int sample_most(int vocab, int ctas, int threads) {
-  const int room = sample_seg<T>(vocab, ctas, threads) * (threads / 32);
+int sample_most(int vocab, bool aligned, int ctas, int threads) {
+  const int room = sample_seg<T>(vocab, aligned, ctas, threads) * (threads / 32);
   return room < vocab ? room : vocab;
 }
 
 template <typename T>
-SamplePlan sample_plan(int rows, int vocab) {
+SamplePlan sample_plan(int rows, int vocab, bool aligned) {
   // CTAs of a row: as many as leave all rows' clusters resident, while a CTA has a few thousand values. Not more where
   // a CTA's part then does not fit its shared memory: 64 rows of 151936 in 32 bits with 4 CTAs in two waves / 2
   // CTAs that read the row from L2 in each pass, us: top-k 33 / 23, top-p 71 / 62.
   SamplePlan p;
   p.ctas = 1;
   while (p.ctas < SM_CTAS && vocab / (p.ctas * 2) >= 3000 && rows <= sample_resident(p.ctas * 2)) p.ctas *= 2;
-  // (stretches are rounded up to whole vectors: a CTA may get more than its share of the row)
-  while (sample_most<T>(vocab, p.ctas, SM_THREADS) > SM_MOST) p.ctas *= 2;
+  // (Stretches are rounded up to whole vectors: a CTA may get more than its share of the row. Aligned rows of 2^17, 2^18 and
+  // 2^19 just do with as few CTAs: 64 rows of 2^18 in 16 bits with 2 CTAs / 4 in two waves, us: top-k 20 / 31, min-p 17 / 23,
+  // but top-p 276 / 194.)
+  while (sample_most<T>(vocab, aligned, p.ctas, SM_THREADS) > SM_MOST) p.ctas *= 2;
   // Fewer threads meet faster, more hide the latency of the 64-bit arithmetic. 512 / 1024 threads, us: 1 row of 151936
   // (19000 a CTA) top-p 22.7 / 25.1, 7 of 32003 top-k 10.7 / 11.4; 32 of 151936 (38000 a CTA) top-p 35.5 / 34.1.
   p.threads = vocab / p.ctas < 24000 ? 512 : SM_THREADS;
-  p.seg = sample_seg<T>(vocab, p.ctas, p.threads);
+  p.seg = sample_seg<T>(vocab, aligned, p.ctas, p.threads);
   return p;
 }
 
@@ -1099,21 +1101,23 @@ int sample_launch(SampleArgs a, int rows, int ctas, cudaStream_t stream) {
 
 template <typename T>
 int sample_go(SampleArgs a, int rows, cudaStream_t stream) {
-  const SamplePlan p = sample_plan<T>(rows, a.vocab);
+  const bool aligned = (uintptr_t)a.x % 16 == 0 && (rows == 1 || a.stride % Vec<T>::N == 0);
+  const SamplePlan p = sample_plan<T>(rows, a.vocab, aligned);
   a.seg = p.seg;
   return p.threads == 512 ? sample_launch<T, 512>(a, rows, p.ctas, stream) : sample_launch<T, 1024>(a, rows, p.ctas, stream);
 }
 
 }  // namespace
 
-extern "C" int q_sample_tokens_plan(int fp32, int rows, int vocab, int* ctas, int* values) {
+extern "C" int q_sample_tokens_plan(int fp32, int rows, int vocab, int aligned, int* ctas, int* values) {
   const char* who = "q_sample_tokens_plan";
   Q_CHECK_ARG(ctas && values, "%s: null pointer", who);
   Q_CHECK_ARG(rows >= 1 && rows <= SM_MAX_ROWS && vocab >= 1 && vocab <= SM_MAX_VOCAB,
               "%s: %d rows of %d values (1 to 2^24 rows of up to %d)", who, rows, vocab, SM_MAX_VOCAB);
-  const SamplePlan p = fp32 ? sample_plan<float>(rows, vocab) : sample_plan<bf16>(rows, vocab);
+  const bool al = aligned != 0;
+  const SamplePlan p = fp32 ? sample_plan<float>(rows, vocab, al) : sample_plan<bf16>(rows, vocab, al);
   *ctas = p.ctas;
-  *values = fp32 ? sample_most<float>(vocab, p.ctas, p.threads) : sample_most<bf16>(vocab, p.ctas, p.threads);
+  *values = fp32 ? sample_most<float>(vocab, al, p.ctas, p.threads) : sample_most<bf16>(vocab, al, p.ctas, p.threads);
   return Q_OK;
 }
 

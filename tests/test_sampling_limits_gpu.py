@@ -20,10 +20,11 @@ def ops():
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows,vocab", [(64, 262144), (34, 524288), (130, 131072)])
-def test_long_rows_of_equal_values(ops, dtype, rows, vocab):
+@pytest.mark.parametrize("before", [0, 1])
+def test_long_rows_of_equal_values(ops, dtype, rows, vocab, before):
     """All logits but one are equal, and a piece of 15 bits of their weight is nearly 2^15: 32715 and 32740, so that
     131284 and 131184 of them pass 2^32. Top-p cuts through the equal ones."""
-    x = torch.full((rows, vocab), -0.419921875, dtype=dtype, device="cuda")
+    x = torch.full((rows, vocab + before), -0.419921875, dtype=dtype, device="cuda")[:, before:]
     x[1::2] = -0.42578125
     x[:, vocab - 5] = 0
     u = (torch.arange(rows) + 0.53) / rows
